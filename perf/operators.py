@@ -129,30 +129,21 @@ def run(state):
 
 
 # ---- the framework's calls ---------------------------------------------------------------------
-def _framework():
-    """The package, imported on the first pass as a program does at its start."""
-    global _package
-    if _package is None:
-        sys.path.insert(0, os.path.join(os.getcwd(), "coda-gqa-l_b200"))
-        import coda_gqa_l_b200
-        _package = coda_gqa_l_b200
-    return _package
-
-
-_package = None
-
-
 def _own(s):
-    f = _framework()
+    package = os.path.join(os.getcwd(), "coda-gqa-l_b200")
+    if package not in sys.path:
+        sys.path.insert(0, package)
+    from coda_gqa_l_b200 import Int8Rows, add_rms_norm, int8_linear, quantize_int8
+
     if s["op"] == "norm":
-        y, h = f.add_rms_norm(s["x"], s["w"], residual=s["r"], eps=EPS, int8=s["int8"])
+        y, h = add_rms_norm(s["x"], s["w"], residual=s["r"], eps=EPS, int8=s["int8"])
         out = {"values": y.dequantize(torch.bfloat16), "scale": y.scale} if s["int8"] else {"y": y}
         return {**out, "h": h} if s["residual"] else out
     if s["op"] == "quant":
-        q = f.quantize_int8(s["x"])
+        q = quantize_int8(s["x"])
         return {"values": q.dequantize(torch.bfloat16), "scale": q.scale}
-    return f.int8_linear(f.Int8Rows(s["x"], s["x_scale"]), f.Int8Rows(s["w"], s["w_scale"]), s["b"], residual=s["r"],
-                         dtype=TYPES[s["dtype"]])
+    return int8_linear(Int8Rows(s["x"], s["x_scale"]), Int8Rows(s["w"], s["w_scale"]), s["b"], residual=s["r"],
+                       dtype=TYPES[s["dtype"]])
 
 
 # ---- the plain forms ----------------------------------------------------------------------------
