@@ -69,10 +69,11 @@ class Int8Rows(NamedTuple):
 
 
 def quantize_int8(x: torch.Tensor) -> Int8Rows:
-    """Rows of ``x`` (..., K) in 8 bits: a row's scale is its largest magnitude over 127, its values are rounded to the
-    nearest multiple of that (ties to even).  A row whose largest magnitude is under 2^-100 becomes zeros with scale 0; a
-    row that holds a NaN or an infinity gets scale NaN, and NaN is what any product with it is.  For activations (a row
-    is a token) and, once, for a ``nn.Linear`` weight (a row is an output channel)."""
+    """Rows of ``x`` (..., K) in 8 bits: a row's scale is its largest magnitude over 127 (rounded to float32), its values
+    are the integers nearest to 127 times an element over that magnitude, ties to even.  A row whose largest magnitude is
+    under 2^-100 becomes zeros with scale 0; a row that holds a NaN or an infinity gets scale NaN, and NaN is what any
+    product with it is.  For activations (a row is a token) and, once, for a ``nn.Linear`` weight (a row is an output
+    channel)."""
     return Int8Rows(*_calls().quantize_int8(x))
 
 

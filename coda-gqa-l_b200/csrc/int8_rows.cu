@@ -2,7 +2,7 @@
 //
 //   s = x + residual                        (written in the type of x: the residual stream)
 //   y = s * rsqrt(mean(s^2) + eps) * weight (of the unrounded s)
-//   out = y rounded to the type of x, or in 8 bits:  a = max|y|,  scale = a / 127,  q = rint(y * (127 / a))
+//   out = y rounded to the type of x, or in 8 bits:  a = max|y|,  scale = a / 127,  q = rint(127 y / a), ties to even
 //
 // Everything between the loads and the stores is fp32, each output is rounded once.  A row whose largest magnitude is
 // under 2^-100 becomes zeros with scale 0 (127 / a would leave fp32's range); a row that holds a NaN or an infinity
@@ -66,16 +66,70 @@ template <typename T, int EPC> __device__ __forceinline__ void st_chunk(T* p, co
     else *reinterpret_cast<uint32_t*>(p) = w[0];
   }
 }
-__device__ __forceinline__ int q8(float y, float inv) { return __float2int_rn(y * inv); }
-template <int EPC> __device__ __forceinline__ void st_q(int8_t* p, const float (&v)[EPC], float inv) {
-  if constexpr (EPC == 1) *p = (int8_t)q8(v[0], inv);
-  else if constexpr (EPC == 2) *reinterpret_cast<uint16_t*>(p) = (uint16_t)((q8(v[0], inv) & 0xff) | (q8(v[1], inv) & 0xff) << 8);
+// What 8-bit row a largest magnitude (its bits: NaN and infinity are the largest) makes: scale, and the factor to 127.
+// (inv is 0 where the row becomes zeros)
+struct Q8 { float a, scale, inv; };
+__device__ __forceinline__ Q8 row_scale(uint32_t amax) {
+  const float a = __uint_as_float(amax);
+  if (amax >= 0x7f800000u) return Q8{0.f, __uint_as_float(0x7fc00000u), 0.f};
+  if (a < 7.888609e-31f) return Q8{0.f, 0.f, 0.f};
+  return Q8{a, __fdiv_rn(a, 127.f), __fdiv_rn(127.f, a)};
+}
+// q = rint(127 y / a), ties to even.  To round, 1.5 * 2^23 is added: its last bit is worth 1, and the low byte of the sum's
+// bits is q.  y * inv is within 127 * 2^-24 of the quotient, so its nearest integer is right unless it lies that close to a
+// half.  A row's largest value being even, half of it is such a tie: without more, 1 of some 6000 values of random bf16 rows
+// came out a step off (and 1 of 20000 by a division by the scale: two roundings miss ties too).  How far that is looked at:
+// Q8_SHORT  bf16 rows as they are: a quotient of two 8-bit values is a half or 2 / (512 * 255) away from one at the least (254 y -
+//           256 a is even; further above one half), so y * inv is rounded to multiples of 2^-15 first: that restores the
+//           halves and makes none.
+// Q8_LONG   float32 rows as they are: near a half 127 y is compared with the half's multiple of a, in products split into two
+//           floats each, by a call: 1 of 50000 random values is that near (8192 x 4096: 26.9 us, 25.9 without; 28.7 with the
+//           comparison for every value).
+// Q8_PLAIN  normed rows, whose y has roundings of its own that weigh more.
+enum { Q8_SHORT, Q8_LONG, Q8_PLAIN };
+constexpr float Q8_MAGIC = 12582912.f, Q8_SNAP = 384.f, Q8_NEAR = 0.49999f;
+__device__ __noinline__ float q8_near_half(float y, float q, float d, float a) {   // y * inv = q + d
+  const float k = a > 1.f ? 0.00390625f : 1.f, c = 127.f * k;                     // (127 y of rows near the end of the range)
+  a *= k;
+  const float h = q + copysignf(0.5f, d), p = y * c, s = h * a;
+  const float over = (p - s) + (fmaf(y, c, -p) - fmaf(h, a, -s));                 // 127 y - h a: p - s is exact, both rests are
+  return over > 0.f ? h + 0.5f : over < 0.f ? h - 0.5f : rintf(h);
+}
+// Elements of a row that hold y to 8 bits, in the low bytes of w[i].
+template <int EPC, int KIND> __device__ __forceinline__ void to_q8(const float (&v)[EPC], const Q8& r, uint32_t (&w)[EPC]) {
+  if (r.inv == 0.f) {                                                              // (0 * infinity would be no zero)
+#pragma unroll
+    for (int i = 0; i < EPC; ++i) w[i] = 0u;
+    return;
+  }
+  float far = 0.f;
+#pragma unroll
+  for (int i = 0; i < EPC; ++i) {
+    if constexpr (KIND == Q8_SHORT) w[i] = __float_as_uint(fmaf(v[i], r.inv, Q8_SNAP) + (Q8_MAGIC - Q8_SNAP));
+    else {
+      const float g = fmaf(v[i], r.inv, Q8_MAGIC);
+      if constexpr (KIND == Q8_LONG) far = fmaxf(far, fabsf(fmaf(v[i], r.inv, Q8_MAGIC - g)));
+      w[i] = __float_as_uint(g);
+    }
+  }
+  if (KIND == Q8_LONG && far > Q8_NEAR) {
+#pragma unroll
+    for (int i = 0; i < EPC; ++i) {
+      const float q = __uint_as_float(w[i]) - Q8_MAGIC, d = fmaf(v[i], r.inv, -q);
+      if (fabsf(d) > Q8_NEAR) w[i] = __float_as_uint(q8_near_half(v[i], q, d, r.a) + Q8_MAGIC);
+    }
+  }
+}
+template <int EPC, int KIND> __device__ __forceinline__ void st_q(int8_t* p, const float (&v)[EPC], const Q8& r) {
+  uint32_t b[EPC];
+  to_q8<EPC, KIND>(v, r, b);
+  if constexpr (EPC == 1) *p = (int8_t)b[0];
+  else if constexpr (EPC == 2) *reinterpret_cast<uint16_t*>(p) = (uint16_t)__byte_perm(b[0], b[1], 0x40);
   else {
     uint32_t w[EPC / 4];
 #pragma unroll
     for (int i = 0; i < EPC / 4; ++i)
-      w[i] = (uint32_t)(q8(v[4 * i], inv) & 0xff) | (uint32_t)(q8(v[4 * i + 1], inv) & 0xff) << 8 |
-             (uint32_t)(q8(v[4 * i + 2], inv) & 0xff) << 16 | (uint32_t)(q8(v[4 * i + 3], inv) & 0xff) << 24;
+      w[i] = __byte_perm(__byte_perm(b[4 * i], b[4 * i + 1], 0x40), __byte_perm(b[4 * i + 2], b[4 * i + 3], 0x40), 0x5410);
     if constexpr (EPC == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
     else *reinterpret_cast<uint32_t*>(p) = w[0];
   }
@@ -122,14 +176,6 @@ template <bool CTA> __device__ __forceinline__ uint32_t row_max(uint32_t v, uint
     v = __reduce_max_sync(0xffffffffu, (int)(threadIdx.x & 31) < n ? sh[threadIdx.x & 31] : 0u);
   }
   return v;
-}
-
-// What 8-bit row a largest magnitude (its bits: NaN and infinity are the largest) makes: scale, and the factor to 127.
-__device__ __forceinline__ void row_scale(uint32_t amax, float& scale, float& inv) {
-  const float a = __uint_as_float(amax);
-  if (amax >= 0x7f800000u) { scale = __uint_as_float(0x7fc00000u); inv = 0.f; }
-  else if (a < 7.888609e-31f) { scale = 0.f; inv = 0.f; }
-  else { scale = __fdiv_rn(a, 127.f); inv = __fdiv_rn(127.f, a); }
 }
 
 // The row in registers: thread t of the row's TPR threads holds chunks t, t + TPR, ... (NCH of them, EPC elements each).
@@ -203,23 +249,20 @@ __global__ void __launch_bounds__(THREADS) int8_rows_kernel(RowsParams p) {
   for (int j = 0; j < NCH; ++j)
 #pragma unroll
     for (int i = 0; i < EPC; ++i) amax = max(amax, __float_as_uint(v[j][i]) & 0x7fffffffu);
-  float scale, inv;
-  row_scale(row_max<CTA>(amax, sh_max), scale, inv);
-  const bool zero = inv == 0.f;          // (0 * infinity would be no zero)
+  const Q8 to = row_scale(row_max<CTA>(amax, sh_max));
   int8_t* q = p.q + row * p.q_rs;
+  constexpr int KIND = NORM ? Q8_PLAIN : sizeof(T) == 2 ? Q8_SHORT : Q8_LONG;
 #pragma unroll
   for (int j = 0; j < NCH; ++j) {
     const int at = first(j);
-    if (zero) {
-#pragma unroll
-      for (int i = 0; i < EPC; ++i) v[j][i] = 0.f;
-    }
     if constexpr (STAGGER) {
-      if (at >= 0 && at < p.dim) q[at] = (int8_t)q8(v[j][0], inv);
-      if (at + 1 < p.dim) q[at + 1] = (int8_t)q8(v[j][1], inv);
-    } else if (at < p.dim) st_q<EPC>(q + at, v[j], inv);
+      uint32_t b[EPC];
+      to_q8<EPC, KIND>(v[j], to, b);
+      if (at >= 0 && at < p.dim) q[at] = (int8_t)b[0];
+      if (at + 1 < p.dim) q[at + 1] = (int8_t)b[1];
+    } else if (at < p.dim) st_q<EPC, KIND>(q + at, v[j], to);
   }
-  if (t == 0) p.scale[row] = scale;
+  if (t == 0) p.scale[row] = to.scale;
 }
 
 // Rows longer than the registers of a CTA hold: the same in three passes, re-read from L2 where they fit it.
@@ -240,16 +283,20 @@ __global__ void __launch_bounds__(1024) int8_rows_long_kernel(RowsParams p) {
     inv = rsqrtf(__fdiv_rn(row_sum<true>(ss, sh_sum), (float)p.dim) + p.eps);
   }
   auto normed = [&](float s, int d) { return w != nullptr ? s * inv * El<T>::ld(w + d) : s; };
-  float scale = 0.f, to = 0.f;
+  Q8 to{};
   if (p.q != nullptr) {
     uint32_t amax = 0;
     for (int d = threadIdx.x; d < p.dim; d += blockDim.x) amax = max(amax, __float_as_uint(normed(at(d), d)) & 0x7fffffffu);
-    row_scale(row_max<true>(amax, sh_max), scale, to);
-    if (threadIdx.x == 0) p.scale[row] = scale;
+    to = row_scale(row_max<true>(amax, sh_max));
+    if (threadIdx.x == 0) p.scale[row] = to.scale;
   }
   for (int d = threadIdx.x; d < p.dim; d += blockDim.x) {
     const float s = at(d), y = normed(s, d);          // (sum may be x or residual itself: each element is read before it is written)
-    if (p.q != nullptr) p.q[row * p.q_rs + d] = to == 0.f ? (int8_t)0 : (int8_t)q8(y, to);
+    if (p.q != nullptr) {
+      const float one[1] = {y};
+      if (w != nullptr) st_q<1, Q8_PLAIN>(p.q + row * p.q_rs + d, one, to);
+      else st_q<1, sizeof(T) == 2 ? Q8_SHORT : Q8_LONG>(p.q + row * p.q_rs + d, one, to);
+    }
     else El<T>::st((T*)p.y + row * p.y_rs + d, y);
     if (p.sum != nullptr) El<T>::st((T*)p.sum + row * p.sum_rs + d, s);
   }

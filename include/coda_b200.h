@@ -442,8 +442,9 @@ int coda_b200_route_block_noalloc(const coda_layer_cfg* cfg, const coda_state_pt
  * rows of whole 16-byte vectors are faster).  Sums and norms are fp32, every output is rounded once.
  *   s = x + residual;  sum = s rounded;  y = s * rsqrt(mean(s^2) + eps) * weight  (of the unrounded s)
  * residual and sum are given together or both NULL (sum may be x or residual itself); the normed rows leave either as y
- * (dtype) or as q and scale, the 8-bit form:  a = max |y|, scale = a / 127, q = rint(y / scale).  A row with a < 2^-100
- * gets q = 0, scale = 0; a row with a NaN or an infinity gets q = 0, scale = NaN. */
+ * (dtype) or as q and scale, the 8-bit form:  a = max |y|, scale = a / 127, q = 127 y / a
+ * rounded once, to the nearest integer, ties to even (y as computed: a normed row's fp32 values).  A row with a < 2^-100 gets q = 0, scale = 0; a row with a NaN or an
+ * infinity gets q = 0, scale = NaN. */
 int coda_b200_add_rms_norm(int32_t dtype, int64_t rows, int32_t dim, const void* x, int64_t x_rs,
                            const void* residual, int64_t res_rs, const void* weight, float eps,
                            void* sum, int64_t sum_rs, void* y, int64_t y_rs,

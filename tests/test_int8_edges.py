@@ -1,0 +1,49 @@
+"""The 8-bit operators at the edges of what they are documented to take: values that lie on a tie, single rows of odd length,
+scales far from one, inputs that carry a tangent, and calls under a tracer or a dispatch mode."""
+import pytest
+import torch
+
+from tests.test_int8 import DTYPES, U, gen, half_step, randn, rows_int8
+
+
+def assert_nearest(x, q):
+    """``q`` holds the integers nearest to 127 x / a, ties to even, a the row's largest magnitude.  Checked in integers: with
+    at most 24 bits in x and a, 254 x and 2 q a have 32 each, and where q is not 0 their exponents differ by at most nine, so
+    that float64 holds both and their difference exactly (where q is 0 the difference is 254 x itself)."""
+    a = x.double().abs().amax(-1, keepdim=True)
+    v = q.values.double()
+    off = (254 * x.double() - 2 * v * a).abs()
+    assert bool((off <= a).all()), int((off > a).sum())
+    tie = (off == a) & (a > 0)
+    assert bool((q.values[tie] % 2 == 0).all()), int((q.values[tie] % 2 != 0).sum())
+    return int(tie.sum())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [16, 33, 1000, 4096, 40960])
+def test_values_on_a_tie_and_near_one(dim, dtype):
+    """Rows whose largest value is each bfloat16 mantissa and which hold half of it (an exact tie at 63.5), rows of multiples
+    of a 254th of their largest (every value a tie or an integer) and their neighbours in the type, at sizes over the range."""
+    from coda_gqa_l_b200 import quantize_int8
+    g = gen(dim)
+    rows = []
+    for scale in (1.0, 2.0 ** -92, 2.0 ** 116):
+        r = randn(g, 128, dim)
+        a = torch.arange(128, 256, device="cuda").float()
+        r = r / r.abs().amax(1, keepdim=True) * a[:, None] * 0.99
+        r[:, 0], r[:, 1], r[:, dim // 2], r[:, -1] = a, a / 2, -a / 2, a / 2
+        rows.append(r * scale)
+        n = torch.arange(1, 9, device="cuda").float()[:, None]                    # a = 127 n: ties at odd multiples of n / 2
+        h = torch.randint(-254, 255, (8, dim), generator=g, device="cuda").float() / 2 * n
+        h[:, 0] = 127 * n[:, 0]
+        rows.append(h * scale)
+    x = torch.cat(rows).to(dtype)
+    assert assert_nearest(x, quantize_int8(x)) > 3 * 128 * 3
+    if dtype == torch.float32:
+        near = torch.cat([x.nextafter(torch.full_like(x, s * 3e38)) for s in (1, -1)])
+        near[:, 0] = torch.cat([x[:, 0]] * 2)                                      # (the largest stays the largest)
+        near = near.clamp(-near[:, :1], near[:, :1])
+        assert_nearest(near, quantize_int8(near))
+    r = randn(g, 300, dim, dtype=dtype)
+    assert_nearest(r, quantize_int8(r))
