@@ -351,10 +351,12 @@ int dispatch_rows(const RowsParams& p, cudaStream_t s) {
 // q * scale, rounded to T.  A thread takes the same E elements of DQ_ROWS rows, all of them requested before the first is used.
 // WHOLE: E elements make 16 bytes of the output, rows of it start on such a boundary.  Else a warp's 256 elements of a row go
 // through shared memory, so that its stores are neighbouring words all the same (8192 x 4095 bf16: 61 us an element a thread,
-// 29 us so; 18 us is what whole rows of about that size take).
+// 29 us so; 18 us is what whole rows of about that size take).  No pointer is __restrict__: the kernel ahead may still be writing q and
+// scale when this one starts, and they must not pass for memory that is constant for its lifetime (loads ahead of the wait,
+// or on the path that is not kept coherent).
 template <typename T, int E, bool WHOLE, int DQ_ROWS>
-__global__ void __launch_bounds__(256) dequantize_rows_kernel(long long rows, int dim, const int8_t* __restrict__ q, long long q_rs,
-                                                              const float* __restrict__ scale, T* __restrict__ out, long long out_rs,
+__global__ void __launch_bounds__(256) dequantize_rows_kernel(long long rows, int dim, const int8_t* q, long long q_rs,
+                                                              const float* scale, T* out, long long out_rs,
                                                               int lanes) {
   __shared__ alignas(16) T seg[WHOLE ? 1 : 8][WHOLE ? 1 : 32 * E];
   const int local = threadIdx.x / lanes, per = blockDim.x / lanes, t = threadIdx.x - local * lanes;

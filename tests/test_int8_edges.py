@@ -47,3 +47,21 @@ def test_values_on_a_tie_and_near_one(dim, dtype):
         assert_nearest(near, quantize_int8(near))
     r = randn(g, 300, dim, dtype=dtype)
     assert_nearest(r, quantize_int8(r))
+
+
+@pytest.mark.gpu
+def test_rows_written_and_read_back_to_back_through_the_same_memory():
+    """Each call reads what the one before it on the stream has just written where the call before that one wrote something
+    else: scales and values never come from an earlier round."""
+    from coda_gqa_l_b200 import quantize_int8
+    g = gen(17)
+    for rows, dim, dtype in ((1, 64, torch.float32), (40, 1000, torch.bfloat16), (300, 512, torch.bfloat16), (2000, 4096, torch.bfloat16)):
+        xs = [randn(g, rows, dim, dtype=dtype) * 4.0 ** i for i in range(5)]
+        want = [quantize_int8(x).dequantize(dtype).clone() for x in xs]
+        torch.cuda.synchronize()
+        bad = torch.zeros((), device="cuda", dtype=torch.int64)
+        for i in range(200):
+            q = quantize_int8(xs[i % 5])
+            bad += (q.dequantize(dtype) != want[i % 5]).sum()
+            del q
+        assert int(bad) == 0
