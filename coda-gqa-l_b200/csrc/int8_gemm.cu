@@ -606,6 +606,9 @@ extern "C" int coda_b200_int8_gemm(int32_t dtype, int32_t M, int32_t K, int32_t 
   CODA_REQUIRE(x && x_scale && w && w_scale && y, CODA_ERR_ARG, "int8_gemm: null pointer");
   CODA_REQUIRE(((uintptr_t)x | (uintptr_t)w) % 16 == 0 && x_rs % 16 == 0 && w_rs % 16 == 0, CODA_ERR_ARG,
                "int8_gemm: rows of x and w must start on 16-byte boundaries");
+  CODA_REQUIRE(((uintptr_t)y | (uintptr_t)bias | (uintptr_t)residual) % (dtype == CODA_F32 ? 4 : 2) == 0 &&
+               ((uintptr_t)x_scale | (uintptr_t)w_scale | (uintptr_t)status) % 4 == 0, CODA_ERR_ARG,
+               "int8_gemm: tensors must start on a boundary of their elements");
   CODA_REQUIRE(x_rs >= K && w_rs >= K && y_rs >= N && (residual == nullptr || res_rs >= N), CODA_ERR_ARG,
                "int8_gemm: row strides shorter than a row");
   Int8GemmParams p = {};

@@ -428,6 +428,9 @@ __global__ void __launch_bounds__(256) dequantize_rows_kernel(long long rows, in
 }  // namespace
 
 static bool known_dtype(int32_t dtype) { return dtype == CODA_F32 || dtype == CODA_BF16; }
+// The addresses (or nulls) lie on boundaries of elements of that size: any other access would end the context.
+template <typename... P> static bool on_elements(uintptr_t bytes, const P*... p) { return (((uintptr_t)p | ... | 0) % bytes) == 0; }
+static uintptr_t size_of(int32_t dtype) { return dtype == CODA_F32 ? 4 : 2; }
 
 extern "C" int coda_b200_add_rms_norm(int32_t dtype, int64_t rows, int32_t dim, const void* x, int64_t x_rs,
                                       const void* residual, int64_t res_rs, const void* weight, float eps,
@@ -438,6 +441,8 @@ extern "C" int coda_b200_add_rms_norm(int32_t dtype, int64_t rows, int32_t dim, 
   if (rows == 0) return CODA_OK;
   CODA_REQUIRE(x && weight && (residual == nullptr) == (sum == nullptr), CODA_ERR_ARG,
                "add_rms_norm: null pointer (sum and residual are given together)");
+  CODA_REQUIRE(on_elements(size_of(dtype), x, residual, weight, sum, y) && on_elements(4, scale), CODA_ERR_ARG,
+               "add_rms_norm: tensors must start on a boundary of their elements");
   CODA_REQUIRE((y != nullptr) != (q != nullptr) && (q != nullptr) == (scale != nullptr), CODA_ERR_ARG,
                "add_rms_norm: give either y, or q and scale");
   CODA_REQUIRE(rows == 1 || ((sum == nullptr || sum_rs >= dim) && (y == nullptr || y_rs >= dim) && (q == nullptr || q_rs >= dim)), CODA_ERR_ARG,
@@ -453,6 +458,7 @@ extern "C" int coda_b200_quantize_rows(int32_t dtype, int64_t rows, int32_t dim,
   CODA_REQUIRE(rows <= 0x7fffffffLL && dim <= 1 << 30, CODA_ERR_LIMIT, "quantize_rows: more than 2^31 - 1 rows, or rows longer than 2^30");
   if (rows == 0) return CODA_OK;
   CODA_REQUIRE(x && q && scale, CODA_ERR_ARG, "quantize_rows: null pointer");
+  CODA_REQUIRE(on_elements(size_of(dtype), x) && on_elements(4, scale), CODA_ERR_ARG, "quantize_rows: tensors must start on a boundary of their elements");
   CODA_REQUIRE(rows == 1 || q_rs >= dim, CODA_ERR_ARG, "quantize_rows: rows of q overlap");
   RowsParams p{rows, dim, x, x_rs, nullptr, 0, nullptr, 0.f, nullptr, 0, nullptr, 0, q, q_rs, scale};
   return dtype == CODA_F32 ? dispatch_rows<float>(p, (cudaStream_t)stream) : dispatch_rows<bf16>(p, (cudaStream_t)stream);
@@ -482,6 +488,7 @@ extern "C" int coda_b200_dequantize_rows(int32_t dtype, int64_t rows, int32_t di
   CODA_REQUIRE(rows <= 0x7fffffffLL && dim <= 1 << 30, CODA_ERR_LIMIT, "dequantize_rows: more than 2^31 - 1 rows, or rows longer than 2^30");
   if (rows == 0) return CODA_OK;
   CODA_REQUIRE(q && scale && out, CODA_ERR_ARG, "dequantize_rows: null pointer");
+  CODA_REQUIRE(on_elements(size_of(dtype), out) && on_elements(4, scale), CODA_ERR_ARG, "dequantize_rows: tensors must start on a boundary of their elements");
   CODA_REQUIRE((uintptr_t)q % 8 == 0 && q_rs % 8 == 0 && q_rs >= dim && out_rs >= dim, CODA_ERR_ARG,
                "dequantize_rows: rows of q must start on 8-byte boundaries, rows must not overlap");
   return dtype == CODA_F32 ? launch_dequantize<float>(rows, dim, q, q_rs, scale, (float*)out, out_rs, (cudaStream_t)stream)

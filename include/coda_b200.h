@@ -438,8 +438,8 @@ int coda_b200_route_block_noalloc(const coda_layer_cfg* cfg, const coda_state_pt
                                   const float* eta_logit, coda_stream_t stream);
 
 /* Rows around projections with 8-bit weights and activations (no counterpart upstream).  `dtype` is the type of x,
- * residual, weight, sum and y; row strides are in elements; rows of any length and alignment are taken (16-byte aligned
- * rows of whole 16-byte vectors are faster).  Sums and norms are fp32, every output is rounded once.
+ * residual, weight, sum and y; row strides are in elements; rows of any length that start at an element are taken
+ * (16-byte aligned rows of whole 16-byte vectors are faster); an address between two elements is refused.  Sums and norms are fp32, every output is rounded once.
  *   s = x + residual;  sum = s rounded;  y = s * rsqrt(mean(s^2) + eps) * weight  (of the unrounded s)
  * residual and sum are given together or both NULL (sum may be x or residual itself); the normed rows leave either as y
  * (dtype) or as q and scale, the 8-bit form:  a = max |y|, scale = a / 127, q = 127 y / a

@@ -65,3 +65,30 @@ def test_rows_written_and_read_back_to_back_through_the_same_memory():
             bad += (q.dequantize(dtype) != want[i % 5]).sum()
             del q
         assert int(bad) == 0
+
+
+def test_c_entries_refuse_addresses_between_two_elements():
+    """What a kernel would read or write with accesses of an element's size starts on one's boundary, or the call is refused on
+    the host (a misaligned access would end the context)."""
+    from coda_gqa_l_b200._lib import lib
+    ok, odd, two = 4096, 4097, 4098                                # never read: every call is refused on the host
+
+    def refused(rc):
+        assert rc == -1 and b"boundar" in lib.coda_b200_last_error(), (rc, lib.coda_b200_last_error())
+
+    for dtype, bad in ((1, odd), (0, two), (0, odd)):
+        names = ("x", "r", "w", "sum", "y")
+        for name in names:
+            a = dict.fromkeys(names, ok) | {name: bad}
+            refused(lib.coda_b200_add_rms_norm(dtype, 4, 8, a["x"], 8, a["r"], 8, a["w"], 1e-6, a["sum"], 8, a["y"], 8, None, 0, None, None))
+        refused(lib.coda_b200_quantize_rows(dtype, 4, 8, bad, 8, ok, 16, ok, None))
+        refused(lib.coda_b200_dequantize_rows(dtype, 4, 8, ok, 16, ok, bad, 8, None))
+        for name in ("b", "r", "y"):
+            a = dict(b=ok, r=ok, y=ok) | {name: bad}
+            refused(lib.coda_b200_int8_gemm(dtype, 4, 64, 8, ok, 64, ok, ok, 64, ok, a["b"], a["r"], 8, a["y"], 8, 0, None, None))
+    refused(lib.coda_b200_add_rms_norm(1, 4, 8, ok, 8, None, 0, ok, 1e-6, None, 0, None, 0, ok, 16, two, None))
+    refused(lib.coda_b200_quantize_rows(1, 4, 8, ok, 8, ok, 16, two, None))
+    refused(lib.coda_b200_dequantize_rows(1, 4, 8, ok, 16, two, ok, 8, None))
+    for scales in ((two, ok), (ok, two)):
+        refused(lib.coda_b200_int8_gemm(1, 4, 64, 8, ok, 64, scales[0], ok, 64, scales[1], None, None, 0, ok, 8, 0, None, None))
+    refused(lib.coda_b200_int8_gemm(1, 4, 64, 8, ok, 64, ok, ok, 64, ok, None, None, 0, ok, 8, 0, two, None))
