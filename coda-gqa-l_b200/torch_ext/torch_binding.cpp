@@ -385,6 +385,7 @@ at::IntArrayRef lead(const Tensor& t) { return t.sizes().slice(0, t.dim() - 1); 
 
 Rows int8_rows_of(const Tensor& t) {
   Rows r = rows_of(t);
+  if (r.n <= 1) r.stride = padded(t.size(-1));           // (one row has no distance to a next)
   if (reinterpret_cast<uintptr_t>(r.t.data_ptr()) % 16 != 0 || r.stride % 16 != 0) {
     const Tensor c = empty_rows(t);
     c.copy_(t);

@@ -50,6 +50,40 @@ def test_values_on_a_tie_and_near_one(dim, dtype):
 
 
 @pytest.mark.gpu
+def test_single_rows_of_odd_length_are_used_in_place():
+    """One row has no distance to another: rows of this package's own making are neither copied nor moved, a product allocates
+    its result and nothing else, as it does for two rows."""
+    from coda_gqa_l_b200 import Int8Rows, int8_linear, quantize_int8
+    g = gen(3)
+    w = quantize_int8(randn(g, 40, 577))
+
+    def blocks(call):
+        call()
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_stats()["allocation.all.allocated"]
+        out = call()
+        return torch.cuda.memory_stats()["allocation.all.allocated"] - before, out
+
+    for shape in ((1, 577), (1, 1, 577), (577,), (2, 577)):
+        q = quantize_int8(randn(g, *shape))
+        n, y = blocks(lambda: int8_linear(q, w, dtype=torch.float32))
+        assert n == 1, shape
+        ref = (q.values.double() * q.scale.double()[..., None]) @ (w.values.double() * w.scale.double()[:, None]).t()
+        mag = (q.values.double().abs() * q.scale.double()[..., None]) @ (w.values.double().abs() * w.scale.double()[:, None]).t()
+        assert bool(((y.double() - ref).abs() <= 6 * U * mag).all())
+        n, d = blocks(lambda: q.dequantize(torch.float32))
+        assert n == 1 and torch.equal(d, q.values.float() * q.scale[..., None])
+    # one weight row, and a single row that does not start on a 16-byte boundary (copied)
+    q, one = quantize_int8(randn(g, 3, 577)), quantize_int8(randn(g, 1, 577))
+    n, y = blocks(lambda: int8_linear(q, one, dtype=torch.float32))
+    assert n == 1 and y.shape == (3, 1)
+    buf = torch.zeros(600, device="cuda", dtype=torch.int8)
+    off = buf[3:580].view(1, 577).copy_(one.values)
+    assert torch.equal(int8_linear(q, Int8Rows(off, one.scale), dtype=torch.float32), y)
+    assert torch.equal(Int8Rows(off, one.scale).dequantize(torch.float32), one.dequantize(torch.float32))
+
+
+@pytest.mark.gpu
 def test_rows_written_and_read_back_to_back_through_the_same_memory():
     """Each call reads what the one before it on the stream has just written where the call before that one wrote something
     else: scales and values never come from an earlier round."""
