@@ -1,5 +1,6 @@
 // y[m][n] = x_scale[m] * w_scale[n] * sum_k x[m][k] w[n][k]  (+ bias[n]) (+ residual[m][n]), x and w in 8-bit integers.
-// The sum is exact in 32 bits (K <= 131071: 2^14 * K < 2^31), the rest is fp32, rounded once to the type of y.
+// The sum is exact in 32 bits (K <= 131071: 2^14 * K < 2^31), the rest is fp32, rounded once to the type of y.  The sum is
+// scaled by one factor after the other: the product of both scales may leave fp32's range where the result does not.
 //
 // Both kernels run tcgen05.mma.kind::i8 with the operands swapped: the WEIGHT rows (output channels) are the MMA's M,
 // the tokens its N, so that a decode step's few tokens waste no tensor work, and a thread of the epilogue, which owns a
@@ -257,7 +258,7 @@ int8_split_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constan
     for (int i = 0; i < 8; ++i) r[i] = p.res != nullptr && t + i < nt ? El<T>::ld(s_res + (t + i) * IG_BN + row) : 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (t + i < nt) El<T>::st(y + (t + i) * p.y_rs, (float)acc[i] * (s_sx[t0 + t + i] * sw) + bias + r[i]);
+      if (t + i < nt) El<T>::st(y + (t + i) * p.y_rs, (float)acc[i] * sw * s_sx[t0 + t + i] + bias + r[i]);
   };
   if (S == 1) {
     if (warp >= 2) {
@@ -462,7 +463,7 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant
           }
 #pragma unroll
           for (int t = 0; t < 32; ++t, y += p.y_rs) {
-            const float v1 = (float)(int)v[t] * (s_sx[b][c + t] * sw) + bias;
+            const float v1 = (float)(int)v[t] * sw * s_sx[b][c + t] + bias;
             if (c + t < mt) El<T>::st(y, p.res != nullptr ? v1 + r[t] : v1);
           }
         }

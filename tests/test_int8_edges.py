@@ -84,6 +84,30 @@ def test_single_rows_of_odd_length_are_used_in_place():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,k,n", [(3, 64, 40), (40, 100, 300), (300, 64, 300)])
+def test_scales_whose_product_leaves_the_range(m, k, n, dtype):
+    """A token's scale far below one with a channel's scale below it, and both far above: the product of the two is not a normal
+    number although the result is; and a sum of zero stays zero.  Three roundings as everywhere: u each."""
+    from coda_gqa_l_b200 import Int8Rows, int8_linear
+    g = gen(m)
+    xv, xs = rows_int8(g, m, k)
+    wv, ws = rows_int8(g, n, k)
+    for sx, sw in ((2.0 ** -98, 2.0 ** -30), (2.0 ** -30, 2.0 ** -98), (2.0 ** -98, 2.0 ** -36)):
+        a, b = Int8Rows(xv, (1 + xs * 50) * sx), Int8Rows(wv, (1 + ws * 50) * sw)
+        y = int8_linear(a, b, dtype=dtype)
+        ref = (xv.double() @ wv.double().t()) * a.scale.double()[:, None] * b.scale.double()
+        err = (y.double() - ref).abs()
+        normal = ref.abs() > 2.0 ** -125
+        assert int(normal.sum()) > m * n // 2
+        assert bool((err <= ref.abs() * (4 * U + half_step(dtype)))[normal].all())
+        assert bool((err <= 2.0 ** -133)[~normal].all())
+    zero = torch.zeros_like(xv)
+    y = int8_linear(Int8Rows(zero, torch.full_like(xs, 2.0 ** 100)), Int8Rows(wv, torch.full_like(ws, 2.0 ** 60)), dtype=dtype)
+    assert not bool(y.any()) and not bool(y.isnan().any())
+
+
+@pytest.mark.gpu
 def test_rows_written_and_read_back_to_back_through_the_same_memory():
     """Each call reads what the one before it on the stream has just written where the call before that one wrote something
     else: scales and values never come from an earlier round."""
