@@ -610,6 +610,7 @@ namespace {
 const Tensor& unpack(PyObject* o, const char* what, bool input) {
   TORCH_CHECK_TYPE(THPVariable_Check(o), text("%s: expected a tensor", what));
   const Tensor& t = THPVariable_Unpack(o);
+  TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), text("%s is for inference: it has no derivative (a tensor carries a tangent)", what));
   if (input) {
     TORCH_CHECK(t.is_cuda(), text("%s: input must be a CUDA tensor: this implementation has no CPU path", what));
     if (t.requires_grad() && at::GradMode::is_enabled()) {

@@ -107,6 +107,38 @@ def test_scales_whose_product_leaves_the_range(m, k, n, dtype):
     assert not bool(y.any()) and not bool(y.isnan().any())
 
 
+def calls_with(t):
+    """Every call that takes an activation, with ``t`` applied to that activation; the first one also takes weights."""
+    from coda_gqa_l_b200 import Int8Rows, add_rms_norm, int8_linear, quantize_int8
+    x, w = torch.randn(4, 64, device="cuda"), torch.ones(64, device="cuda")
+    q, p = quantize_int8(x), quantize_int8(torch.randn(8, 64, device="cuda"))
+    res = torch.zeros(4, 8, device="cuda")
+    return (lambda: quantize_int8(t(x)), lambda: add_rms_norm(t(x), w), lambda: add_rms_norm(t(x), w, int8=True),
+            lambda: add_rms_norm(x, w, residual=t(x)), lambda: Int8Rows(q.values, t(q.scale)).dequantize(),
+            lambda: int8_linear(Int8Rows(q.values, t(q.scale)), p), lambda: int8_linear(q, p, residual=t(res), dtype=torch.float32))
+
+
+@pytest.mark.gpu
+def test_inputs_with_a_tangent_are_refused():
+    """The tangent of a dual number, an activation's or a weight's, is refused and not dropped."""
+    import torch.autograd.forward_ad as fa
+
+    from coda_gqa_l_b200 import Int8Rows, add_rms_norm, int8_linear, quantize_int8
+    x, w = torch.randn(4, 64, device="cuda"), torch.ones(64, device="cuda")
+    q, p = quantize_int8(x), quantize_int8(torch.randn(8, 64, device="cuda"))
+    b = torch.zeros(8, device="cuda")
+    with fa.dual_level():
+        dual = lambda t: fa.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (*calls_with(dual), lambda: add_rms_norm(x, dual(w)), lambda: int8_linear(q, Int8Rows(p.values, dual(p.scale))),
+                     lambda: int8_linear(q, p, dual(b), dtype=torch.float32)):
+            with pytest.raises(RuntimeError, match="inference"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="inference"):
+                call()
+        for call in calls_with(lambda t: t):
+            call()
+
+
 @pytest.mark.gpu
 def test_rows_written_and_read_back_to_back_through_the_same_memory():
     """Each call reads what the one before it on the stream has just written where the call before that one wrote something
