@@ -606,27 +606,31 @@ TORCH_LIBRARY_IMPL(coda_b200, Meta, m) {
 // the library is a Python module too (PyInit below), with the five 8-bit operators as plain functions of tensors.
 namespace {
 
-// A tensor argument; an activation (`input`) has to be on the GPU and must not ask for a gradient.
-const Tensor& unpack(PyObject* o, const char* what, bool input) {
+// A tensor argument.  What is computed from (all but WEIGHT) has to be on the GPU and must not ask for a gradient; a weight may
+// be a parameter, and so may the rows that quantize_int8 is given (EITHER: an activation, or a weight to be quantised).
+enum Role { WEIGHT, ACTIVATION, EITHER };
+bool is_parameter(PyObject* o) {
+  PyObject* nn = PyImport_ImportModule("torch.nn");
+  PyObject* cls = nn != nullptr ? PyObject_GetAttrString(nn, "Parameter") : nullptr;
+  const bool yes = cls != nullptr && PyObject_IsInstance(o, cls) == 1;
+  Py_XDECREF(cls);
+  Py_XDECREF(nn);
+  if (PyErr_Occurred()) throw python_error();
+  return yes;
+}
+const Tensor& unpack(PyObject* o, const char* what, Role role) {
   TORCH_CHECK_TYPE(THPVariable_Check(o), text("%s: expected a tensor", what));
   const Tensor& t = THPVariable_Unpack(o);
   TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), text("%s is for inference: it has no derivative (a tensor carries a tangent)", what));
-  if (input) {
+  if (role != WEIGHT) {
     TORCH_CHECK(t.is_cuda(), text("%s: input must be a CUDA tensor: this implementation has no CPU path", what));
-    if (t.requires_grad() && at::GradMode::is_enabled()) {
-      PyObject* nn = PyImport_ImportModule("torch.nn");
-      PyObject* cls = nn != nullptr ? PyObject_GetAttrString(nn, "Parameter") : nullptr;
-      const bool parameter = cls != nullptr && PyObject_IsInstance(o, cls) == 1;
-      Py_XDECREF(cls);
-      Py_XDECREF(nn);
-      if (PyErr_Occurred()) throw python_error();
-      TORCH_CHECK(parameter, text("%s is for inference: it has no gradient (use torch.no_grad())", what));
-    }
+    if (t.requires_grad() && at::GradMode::is_enabled())
+      TORCH_CHECK(role == EITHER && is_parameter(o), text("%s is for inference: it has no gradient (use torch.no_grad())", what));
   }
   return t;
 }
-OptTensor unpack_opt(PyObject* o, const char* what, bool input) {
-  return o == Py_None ? OptTensor() : OptTensor(unpack(o, what, input));
+OptTensor unpack_opt(PyObject* o, const char* what, Role role) {
+  return o == Py_None ? OptTensor() : OptTensor(unpack(o, what, role));
 }
 at::ScalarType unpack_dtype(PyObject* o, const char* what) {
   TORCH_CHECK_TYPE(THPDtype_Check(o), text("%s: unsupported dtype: float32 or bfloat16", what));
@@ -649,14 +653,14 @@ template <typename... T> PyObject* pack(const T&... t) {
 PyObject* py_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   arity(n, 1, "quantize_int8");
-  auto [q, scale] = quantize_int8(unpack(a[0], "quantize_int8", true));
+  auto [q, scale] = quantize_int8(unpack(a[0], "quantize_int8", EITHER));
   return pack(THPVariable_Wrap(std::move(q)), THPVariable_Wrap(std::move(scale)));
   END_HANDLE_TH_ERRORS
 }
 PyObject* py_dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   arity(n, 3, "dequantize");
-  return THPVariable_Wrap(dequantize_int8(unpack(a[0], "dequantize", true), unpack(a[1], "dequantize", false), unpack_dtype(a[2], "dequantize")));
+  return THPVariable_Wrap(dequantize_int8(unpack(a[0], "dequantize", ACTIVATION), unpack(a[1], "dequantize", ACTIVATION), unpack_dtype(a[2], "dequantize")));
   END_HANDLE_TH_ERRORS
 }
 // (x, weight, residual or None, eps, int8) -> (y, sum) or (values, scale, sum); the sum is x itself without a residual
@@ -664,15 +668,15 @@ PyObject* py_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   const char* what = "add_rms_norm";
   arity(n, 5, what);
-  const Tensor& x = unpack(a[0], what, true);
-  const OptTensor residual = unpack_opt(a[2], "add_rms_norm: residual", true);
+  const Tensor& x = unpack(a[0], what, ACTIVATION);
+  const OptTensor residual = unpack_opt(a[2], "add_rms_norm: residual", ACTIVATION);
   const double eps = PyFloat_AsDouble(a[3]);
   if (PyErr_Occurred()) throw python_error();
   TORCH_CHECK_VALUE(eps > 0.0, "add_rms_norm: eps must be positive");
   const int int8 = PyObject_IsTrue(a[4]);
   if (int8 < 0) throw python_error();
   Tensor y, q, scale, sum;
-  norm(x, unpack(a[1], what, false), residual, eps, int8 ? nullptr : &y, int8 ? &q : nullptr, int8 ? &scale : nullptr, &sum);
+  norm(x, unpack(a[1], what, WEIGHT), residual, eps, int8 ? nullptr : &y, int8 ? &q : nullptr, int8 ? &scale : nullptr, &sum);
   PyObject* total = residual.has_value() ? THPVariable_Wrap(std::move(sum)) : Py_NewRef(a[0]);
   return int8 ? pack(THPVariable_Wrap(std::move(q)), THPVariable_Wrap(std::move(scale)), total) : pack(THPVariable_Wrap(std::move(y)), total);
   END_HANDLE_TH_ERRORS
@@ -683,9 +687,9 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   arity(n, 9, what);
   const int ready = PyObject_IsTrue(a[8]);
   if (ready < 0) throw python_error();
-  return THPVariable_Wrap(int8_linear(unpack(a[0], what, true), unpack(a[1], what, false), unpack(a[2], what, false), unpack(a[3], what, false),
-                                      unpack_opt(a[4], what, false), unpack_opt(a[5], "int8_linear: residual", true), unpack_dtype(a[6], what),
-                                      unpack_opt(a[7], what, false), ready != 0));
+  return THPVariable_Wrap(int8_linear(unpack(a[0], what, ACTIVATION), unpack(a[1], what, ACTIVATION), unpack(a[2], what, WEIGHT), unpack(a[3], what, WEIGHT),
+                                      unpack_opt(a[4], what, WEIGHT), unpack_opt(a[5], "int8_linear: residual", ACTIVATION), unpack_dtype(a[6], what),
+                                      unpack_opt(a[7], what, WEIGHT), ready != 0));
   END_HANDLE_TH_ERRORS
 }
 

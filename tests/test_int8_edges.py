@@ -140,6 +140,21 @@ def test_inputs_with_a_tangent_are_refused():
 
 
 @pytest.mark.gpu
+def test_activations_that_need_a_gradient_are_refused():
+    """The scales of 8-bit activations among them, and a parameter too where activations are meant; weights may be parameters."""
+    from coda_gqa_l_b200 import Int8Rows, add_rms_norm, int8_linear, quantize_int8
+    for call in (*calls_with(lambda t: t.clone().requires_grad_()), *calls_with(torch.nn.Parameter)[1:]):
+        with pytest.raises(RuntimeError, match="inference"):
+            call()
+        with torch.no_grad():
+            call()
+    x, w = torch.randn(4, 64, device="cuda"), torch.ones(64, device="cuda")
+    q, p = quantize_int8(torch.nn.Parameter(x)), quantize_int8(torch.randn(8, 64, device="cuda"))
+    add_rms_norm(x, torch.nn.Parameter(w))
+    int8_linear(q, Int8Rows(p.values, torch.nn.Parameter(p.scale)), torch.nn.Parameter(torch.zeros(8, device="cuda")), dtype=torch.float32)
+
+
+@pytest.mark.gpu
 def test_rows_written_and_read_back_to_back_through_the_same_memory():
     """Each call reads what the one before it on the stream has just written where the call before that one wrote something
     else: scales and values never come from an earlier round."""
