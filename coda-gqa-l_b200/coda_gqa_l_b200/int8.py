@@ -22,6 +22,7 @@ from __future__ import annotations
 from typing import Dict, NamedTuple, Optional, Tuple, Union
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 __all__ = ["Int8Rows", "add_rms_norm", "int8_linear", "int8_status", "quantize_int8"]
 
@@ -31,17 +32,38 @@ _native = None
 
 
 class _Ops:
-    """The native module's functions, through the dispatcher."""
+    """The native module's functions, through the dispatcher, with its refusals of derivatives."""
 
     def __init__(self, ns):
-        self.quantize_int8, self.dequantize_int8, self.int8_linear = ns.quantize_int8, ns.dequantize_int8, ns.int8_linear
         self._ns = ns
 
+    @staticmethod
+    def _inference(what, *activations, weights=(), parameter=False):
+        for t in (*activations, *weights):
+            if t is not None and forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} is for inference: it has no derivative (a tensor carries a tangent)")
+        for t in activations:
+            if t is not None and t.requires_grad and torch.is_grad_enabled() and not (parameter and isinstance(t, torch.nn.Parameter)):
+                raise RuntimeError(f"{what} is for inference: it has no gradient (use torch.no_grad())")
+
+    def quantize_int8(self, x):
+        self._inference("quantize_int8", x, parameter=True)
+        return self._ns.quantize_int8(x)
+
+    def dequantize_int8(self, values, scale, dtype):
+        self._inference("dequantize", values, scale)
+        return self._ns.dequantize_int8(values, scale, dtype)
+
     def add_rms_norm(self, x, weight, residual, eps, int8):
+        self._inference("add_rms_norm", x, residual, weights=(weight,))
         if not eps > 0.0:
             raise ValueError("add_rms_norm: eps must be positive")
         out = (self._ns.add_rms_norm_int8 if int8 else self._ns.add_rms_norm)(x, weight, residual, eps)
         return out if residual is not None else (*out[:-1], x)
+
+    def int8_linear(self, x, x_scale, w, w_scale, bias, residual, dtype, status, w_ready):
+        self._inference("int8_linear", x, x_scale, residual, weights=(w, w_scale, bias))
+        return self._ns.int8_linear(x, x_scale, w, w_scale, bias, residual, dtype, status, w_ready)
 
 
 def _calls():

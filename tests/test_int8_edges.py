@@ -154,6 +154,27 @@ def test_activations_that_need_a_gradient_are_refused():
     int8_linear(q, Int8Rows(p.values, torch.nn.Parameter(p.scale)), torch.nn.Parameter(torch.zeros(8, device="cuda")), dtype=torch.float32)
 
 
+def test_gradients_are_refused_under_a_dispatch_mode_too():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from coda_gqa_l_b200 import Int8Rows, add_rms_norm, int8_linear, quantize_int8
+    with FakeTensorMode():
+        x, w = torch.empty(4, 64, device="cuda"), torch.ones(64, device="cuda")
+        q, p = quantize_int8(x), quantize_int8(torch.empty(8, 64, device="cuda"))
+        g = torch.empty(4, 64, device="cuda", requires_grad=True)
+        res = torch.empty(4, 8, device="cuda", requires_grad=True)
+        scale = torch.empty(4, device="cuda", requires_grad=True)
+        for call in (lambda: quantize_int8(g), lambda: add_rms_norm(g, w), lambda: add_rms_norm(g, w, int8=True),
+                     lambda: add_rms_norm(x, w, residual=g), lambda: Int8Rows(q.values, scale).dequantize(),
+                     lambda: int8_linear(Int8Rows(q.values, scale), p), lambda: int8_linear(q, p, residual=res, dtype=torch.float32)):
+            with pytest.raises(RuntimeError, match="inference"):
+                call()
+            with torch.no_grad():
+                call()
+        quantize_int8(torch.nn.Parameter(x))
+        add_rms_norm(x, torch.nn.Parameter(w))
+
+
 @pytest.mark.gpu
 def test_rows_written_and_read_back_to_back_through_the_same_memory():
     """Each call reads what the one before it on the stream has just written where the call before that one wrote something
