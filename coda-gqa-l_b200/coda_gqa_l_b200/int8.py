@@ -14,8 +14,8 @@ captured into a CUDA graph.  Tensors are float32 or bfloat16, as everywhere in t
 
 A call is one native function (torch_ext/torch_binding.cpp: checks, allocation, launch; the C ABI below it is
 ``coda_b200_add_rms_norm`` and its neighbours in include/coda_b200.h), because the rows of a decode step take the GPU less
-time than the host takes to ask for them.  Under a dispatch mode (fake tensors, tracers) the calls go through the
-operators of the same names in ``torch.ops.coda_b200``.
+time than the host takes to ask for them.  Under a dispatch mode (fake tensors, tracers) and under ``torch.jit.trace`` the
+calls go through the operators of the same names in ``torch.ops.coda_b200``.
 """
 from __future__ import annotations
 
@@ -28,6 +28,7 @@ __all__ = ["Int8Rows", "add_rms_norm", "int8_linear", "int8_status", "quantize_i
 
 _STATUS: Dict[int, torch.Tensor] = {}      # per device: code of a bounded wait that expired in int8_linear
 _modes = torch._C._len_torch_dispatch_stack
+_tracing = torch._C._get_tracing_state
 _native = None
 
 
@@ -68,7 +69,7 @@ class _Ops:
 
 def _calls():
     global _native
-    if _modes():
+    if _modes() or _tracing() is not None:
         from . import torch_ops
         return _Ops(torch_ops.load())
     if _native is None:

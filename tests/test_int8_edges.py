@@ -176,6 +176,24 @@ def test_gradients_are_refused_under_a_dispatch_mode_too():
 
 
 @pytest.mark.gpu
+def test_a_traced_call_follows_its_inputs():
+    """torch.jit.trace records the operators, not the values they had."""
+    from coda_gqa_l_b200 import add_rms_norm, int8_linear, quantize_int8
+    g = gen(9)
+    w, nw = quantize_int8(randn(g, 24, 64)), 1 + 0.1 * randn(g, 64)
+
+    def f(x, r):
+        q, h = add_rms_norm(x, nw, residual=r, int8=True)
+        return int8_linear(q, w, dtype=torch.float32), h, quantize_int8(x).dequantize(torch.float32), add_rms_norm(r, nw)[0]
+
+    a, b = [(randn(g, 5, 64), randn(g, 5, 64)) for _ in range(2)]
+    with torch.no_grad():
+        traced = torch.jit.trace(f, a, check_trace=False)
+        for args in (a, b):
+            assert all(torch.equal(p, q) for p, q in zip(traced(*args), f(*args)))
+
+
+@pytest.mark.gpu
 def test_rows_written_and_read_back_to_back_through_the_same_memory():
     """Each call reads what the one before it on the stream has just written where the call before that one wrote something
     else: scales and values never come from an earlier round."""
