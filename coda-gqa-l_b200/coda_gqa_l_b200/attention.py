@@ -68,6 +68,12 @@ def _side_stream_for(device: torch.device) -> "torch.cuda.Stream":
     return st
 
 
+def _recording(t: torch.Tensor) -> bool:
+    """Is what runs on ``t`` now being captured into a CUDA graph?  It has no results before a replay then, each replay runs
+    it again, and its memory is the graph's: nothing made by it is kept for calls outside."""
+    return t.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 def _p(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
@@ -194,6 +200,7 @@ class CoDAGQALandmarkPerf2(nn.Module):
         self._fused = None
         self._fused_ptrs = []
         self._wt = None
+        self._recorded: Dict[int, torch.Tensor] = {}
         # When set to a list, every attention launch appends (Lq, start_event, end_event) to it.
         self.kernel_timers = None
         self._qrec = None
@@ -272,6 +279,8 @@ class CoDAGQALandmarkPerf2(nn.Module):
                 st._exact_v_norm.copy_(F.normalize(st.v_buf[:, :, W:W + Me, :], dim=-1, eps=1e-6))
             if Ms > 0:
                 st._sum_lf_k_norm.copy_(F.normalize(st.k_buf[:, :, W + Me:, self.lf_start:], dim=-1, eps=1e-6))
+        if plain and st.k_buf.is_cuda and not _recording(st.k_buf):
+            self._status_word(st.k_buf.device)     # (before a first call that may be captured: a replay would clear one made there)
         if self.collect_metrics:
             st.metrics = new_metrics(st.active_exact, st.active_summary)
         return st
@@ -472,7 +481,8 @@ class CoDAGQALandmarkPerf2(nn.Module):
                 torch.sin(th).to(device=device, dtype=dtype).contiguous(),
                 self.summary_eta_logit.detach().to(device=device, dtype=torch.float32).contiguous(),
                 None if nw is None else nw.detach().to(device=device, dtype=dtype).contiguous())
-        self._const_cache["k"] = (key, vals)
+        if not _recording(th):
+            self._const_cache["k"] = (key, vals)
         return vals
 
     def _fused_weight(self):
@@ -480,7 +490,9 @@ class CoDAGQALandmarkPerf2(nn.Module):
 
         The individual ``nn.Linear`` parameters are re-pointed at row ranges of the fused matrix (no second
         copy of the weights; ``state_dict`` / ``load_state_dict`` keep working).  Rebuilt whenever a
-        parameter no longer aliases it (after ``.to()``, or when a projection was replaced)."""
+        parameter no longer aliases it (after ``.to()``, or when a projection was replaced).  Where that falls into a
+        graph capture the graph copies the parameters in every replay instead, and the layer keeps the memory they had
+        then, which a later call outside would otherwise free."""
         lins = (self.q_proj, self.k_proj, self.v_proj, self.lambda_proj, self.write_proj)
         if not all(type(l) is nn.Linear for l in lins):
             return None
@@ -500,13 +512,19 @@ class CoDAGQALandmarkPerf2(nn.Module):
         W = torch.zeros((npad, self.embed_dim), device=w0.device, dtype=w0.dtype)
         b = torch.zeros((npad,), device=w0.device, dtype=w0.dtype)
         off = 0
+        recording = _recording(w0)
         for l in lins:
-            W[off:off + l.out_features].copy_(l.weight.data)
-            l.weight.data = W[off:off + l.out_features]
-            if l.bias is not None:
-                b[off:off + l.out_features].copy_(l.bias.data)
-                l.bias.data = b[off:off + l.out_features]
+            for p, to in ((l.weight, W), (l.bias, b)):
+                if p is not None:
+                    to = to[off:off + l.out_features]
+                    to.copy_(p.data)
+                    if recording:
+                        self._recorded[p.data_ptr()] = p.data
+                    else:
+                        p.data = to
             off += l.out_features
+        if recording:
+            return W, b
         self._fused = (W, b)
         self._fused_ptrs = [(l.weight.data_ptr(), None if l.bias is None else l.bias.data_ptr()) for l in lins]
         return self._fused
@@ -530,7 +548,8 @@ class CoDAGQALandmarkPerf2(nn.Module):
         wt = self._wt
         if wt is None or wt[0] != key:
             wt = (key, f[0].t().contiguous(), self.o_proj.weight.detach().t().contiguous())
-            self._wt = wt
+            if not _recording(f[0]):
+                self._wt = wt
         return wt
 
     def refresh_weights(self) -> None:
@@ -552,9 +571,8 @@ class CoDAGQALandmarkPerf2(nn.Module):
         w = self._int8
         if w is None or w[0] != key:
             w = [key, quantize_int8(f[0]), quantize_int8(self.o_proj.weight.detach()), f[1], [False, False]]
-            if f[0].is_cuda and torch.cuda.is_current_stream_capturing():
-                return w                       # (made by the replays, in the graph's own memory: not for calls outside it)
-            self._int8 = w
+            if not _recording(f[0]):
+                self._int8 = w
         return w
 
     def _int8_product(self, rows: Int8Rows, which: int, bias, residual, dtype) -> torch.Tensor:
@@ -674,7 +692,8 @@ class CoDAGQALandmarkPerf2(nn.Module):
                           n_heads_out=c["nq"], n_out=c["n_out"], off_k=c["off_k"], off_v=c["off_v"], off_lam=c["off_lam"],
                           off_gate=c["off_gate"] if c["gated"] else -1)
         c["layer"], c["layer_ptr"] = layer, C.addressof(layer)
-        self.__dict__["_bundle"] = c
+        if not _recording(f[0]):
+            self.__dict__["_bundle"] = c
         return c
 
     def _one_call_ok(self, bd, B: int) -> bool:
@@ -731,10 +750,12 @@ class CoDAGQALandmarkPerf2(nn.Module):
                           off_gate=(nq + 2 * nkv + self.num_heads) * es if self.write_policy != "none" else -1)
         w8 = StepLayerInt8(w_in=w[1][0].data_ptr(), w_in_scale=w[1][1].data_ptr(), w_out=w[2][0].data_ptr(), w_out_scale=w[2][1].data_ptr(),
                            out_bias=_p(ob), w_in_rs=w[1][0].stride(0), w_out_rs=w[2][0].stride(0))
-        c = self.__dict__["_bundle8"] = dict(
+        c = dict(
             dev=device, dt=dtype, w=w, mods=[(n, mods[n]) for n in names], stamps=[(p, p._version, p.data_ptr()) for p in prms],
             layer=layer, w8=w8, layer_ptr=C.addressof(layer), w8_ptr=C.addressof(w8), ws={}, n_out=layer.n_out,
             keep=(inv_freq, cos_t, sin_t, eta, nw, f, ob))
+        if not _recording(f[0]):
+            self.__dict__["_bundle8"] = c
         return c
 
     def _step_eager_int8(self, x, st: CoDAGQALandmarkStatePerf2, residual: Optional[torch.Tensor]) -> Optional[torch.Tensor]:

@@ -1,0 +1,118 @@
+"""Layers and stacks with 8-bit projections on the paths a decoding loop takes (hidden states side by side in memory, with a
+residual, without norms), and what has to happen to the layer's derived weight copies when parameters are replaced, when a
+first call is captured, and when two streams share a layer."""
+import pytest
+import torch
+
+from tests.test_int8 import U, check_int8
+from tests.test_int8_layer import FIELDS, SHAPES, hidden, layer, piecewise, stack
+
+SMALL = SHAPES[0][1]
+BF16 = [s for s in SHAPES if s[0] == torch.bfloat16]
+
+
+def watch_native(mod):
+    """How many eager steps of ``mod`` ran as one native call."""
+    taken = [0]
+    inner = mod._step_eager_int8
+
+    def spy(x, st, residual):
+        y = inner(x, st, residual)
+        taken[0] += y is not None
+        return y
+
+    mod._step_eager_int8 = spy
+    return taken
+
+
+def ring(st):
+    from coda_gqa_l_b200._lib import RingPos
+    return RingPos(int(st.pos), int(st.recent_idx), int(st.recent_filled), None)
+
+
+def on_cpu(monkeypatch=None):
+    """A float32 layer on the CPU, for what the host does with its parameters; rows to 8 bits by their formula."""
+    from coda_gqa_l_b200 import CoDAGQALandmarkPerf2, Int8Rows, attention
+    torch.manual_seed(0)
+    mod = CoDAGQALandmarkPerf2(**SMALL).eval()
+
+    def quantise(x):
+        scale = x.abs().amax(-1) / 127
+        return Int8Rows(torch.round(x / scale[..., None]).to(torch.int8), scale)
+
+    if monkeypatch is not None:
+        monkeypatch.setattr(attention, "quantize_int8", quantise)
+    return mod
+
+
+def test_a_capture_leaves_parameters_and_caches_alone(monkeypatch):
+    """While a graph is captured nothing has been computed yet: parameters are not moved into memory that the graph fills in its
+    replays, no derived copy made then is kept, and the memory that the graph reads the parameters from stays."""
+    from coda_gqa_l_b200 import attention
+    mod = on_cpu(monkeypatch)
+    mod.use_int8_projections = True
+    cpu = torch.device("cpu")
+    where = {n: p.data_ptr() for n, p in mod.named_parameters()}
+    want = torch.cat([l.weight.detach() for l in (mod.q_proj, mod.k_proj, mod.v_proj, mod.lambda_proj, mod.write_proj)])
+    monkeypatch.setattr(attention, "_recording", lambda t: True, raising=False)
+    with torch.no_grad():
+        f = mod._fused_weight()
+        assert torch.equal(f[0][:want.shape[0]], want) and not bool(f[0][want.shape[0]:].any())
+        assert torch.equal(mod._skinny_weights()[1], f[0].t())
+        mod._consts(cpu, torch.float32)
+        mod._decode_bundle(cpu, torch.float32)
+        mod._int8_weights()
+        mod._int8_bundle(cpu, torch.float32)
+        assert where == {n: p.data_ptr() for n, p in mod.named_parameters()}
+        assert mod._fused is None and mod._wt is None and mod._int8 is None and not mod._const_cache
+        assert mod.__dict__.get("_bundle") is None and mod.__dict__.get("_bundle8") is None
+        monkeypatch.setattr(attention, "_recording", lambda t: False)
+        f = mod._fused_weight()                    # outside: the parameters become rows of one matrix, as ever ...
+        assert mod.q_proj.weight.data_ptr() == f[0].data_ptr() != where["q_proj.weight"] and torch.equal(f[0][:want.shape[0]], want)
+        kept = {t.data_ptr(): t for t in mod._recorded.values()}               # ... and what the graph reads is still there
+        for n in ("q_proj", "k_proj", "v_proj", "lambda_proj", "write_proj"):
+            assert torch.equal(kept[where[n + ".weight"]], getattr(mod, n).weight)
+            if getattr(mod, n).bias is not None:
+                assert torch.equal(kept[where[n + ".bias"]], getattr(mod, n).bias)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("int8", [True, False])
+def test_first_call_captured_then_replayed_beside_calls_outside(int8):
+    """A layer whose first call ever is captured: a call outside before the first replay, replays with the memory around them
+    used for other things, a call outside and replays again -- each the result of a layer that was never captured."""
+    from coda_gqa_l_b200 import _deep_copy_state
+    dtype, kw = SHAPES[1]
+    mod, ref = layer(kw, dtype, int8=int8), layer(kw, dtype, int8=int8)
+    x = hidden(2, 40, kw["embed_dim"], dtype, 3)
+    torch.manual_seed(2)
+    s0 = mod.init_state(batch_size=2, device="cuda", dtype=dtype)
+    s1 = _deep_copy_state(s0)
+    arena = s1._arena.clone()
+    run = lambda m, s: m.prefill_chunked(x, s, block_size=16)[0]  # noqa: E731
+
+    def same(a, b):             # (under capture the library may pick another GEMM)
+        assert torch.equal(a, b) if int8 else float((a.double() - b.double()).norm() / b.double().norm()) < 2e-2
+
+    want = run(ref, _deep_copy_state(s0))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(mod, s1)
+    junk = []
+
+    def fill():
+        torch.cuda.synchronize()
+        for p in list(mod.parameters()):
+            junk.extend(torch.full(p.shape, float("nan"), device="cuda", dtype=dtype) for _ in range(3))
+
+    fill()
+    assert torch.equal(run(mod, _deep_copy_state(s0)), want)
+    for _ in range(3):
+        fill()
+        s1._arena.copy_(arena)
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        same(got, want)
+        assert torch.equal(run(mod, _deep_copy_state(s0)), want)
+    assert mod.device_status() == 0
