@@ -542,15 +542,29 @@ class CoDAGQALandmarkPerf2(nn.Module):
         f = self._fused_weight()
         if f is None or type(self.o_proj) is not nn.Linear or self.o_proj.bias is not None:
             return None
-        lins = (self.q_proj, self.k_proj, self.v_proj, self.lambda_proj, self.write_proj)
-        key = (f[0].data_ptr(), f[0]._version, f[1]._version, self.o_proj.weight.data_ptr(), self.o_proj.weight._version,
-               tuple(l.weight._version for l in lins), tuple(-1 if l.bias is None else l.bias._version for l in lins))
         wt = self._wt
-        if wt is None or wt[0] != key:
-            wt = (key, f[0].t().contiguous(), self.o_proj.weight.detach().t().contiguous())
+        if wt is None or not self._made_from(wt[0], f):
+            wt = (self._sources(f), f[0].t().contiguous(), self.o_proj.weight.detach().t().contiguous())
             if not _recording(f[0]):
                 self._wt = wt
         return wt
+
+    def _sources(self, f):
+        """What derived copies of the weights are made from, to be kept beside them: the tensors (which also keeps their
+        memory, so that nothing new comes to lie at an old address) and everyone's version counter."""
+        w = self.o_proj.weight
+        return f, w, w.detach(), self._weight_versions(f)
+
+    def _weight_versions(self, f):
+        lins = (self.q_proj, self.k_proj, self.v_proj, self.lambda_proj, self.write_proj, self.o_proj)
+        return (f[0]._version, f[1]._version, tuple(l.weight._version for l in lins),
+                tuple(-1 if l.bias is None else l.bias._version for l in lins))
+
+    def _made_from(self, sources, f) -> bool:
+        """Are these the sources as they are now?"""
+        w = self.o_proj.weight
+        return (sources[0] is f and sources[1] is w and sources[2].data_ptr() == w.data_ptr()
+                and sources[3] == self._weight_versions(f))
 
     def refresh_weights(self) -> None:
         """Drop the derived weight copies (call after modifying parameters in a way autograd's version counters
@@ -559,18 +573,15 @@ class CoDAGQALandmarkPerf2(nn.Module):
         self._int8 = None
 
     def _int8_weights(self):
-        """[key, fused input weight and output weight in 8 bits, fused bias, used]: quantised on first use and again when an
-        address or version counter of a parameter moves.  ``used``: which of the two has been through a product since, so
+        """[sources, fused input weight and output weight in 8 bits, fused bias, used]: quantised on first use and again when a
+        parameter is another tensor or its version counter moves.  ``used``: which of the two has been through a product since, so
         that the next one may request it ahead of its turn (int8_gemm's ``w_ready``)."""
         f = self._fused_weight()
         if f is None or type(self.o_proj) is not nn.Linear:
             raise RuntimeError("use_int8_projections needs plain nn.Linear projections")
-        lins = (self.q_proj, self.k_proj, self.v_proj, self.lambda_proj, self.write_proj, self.o_proj)
-        key = (f[0].data_ptr(), f[0]._version, f[1]._version, f[0].dtype, self.o_proj.weight.data_ptr(),
-               tuple(l.weight._version for l in lins), tuple(-1 if l.bias is None else l.bias._version for l in lins))
         w = self._int8
-        if w is None or w[0] != key:
-            w = [key, quantize_int8(f[0]), quantize_int8(self.o_proj.weight.detach()), f[1], [False, False]]
+        if w is None or not self._made_from(w[0], f):
+            w = [self._sources(f), quantize_int8(f[0]), quantize_int8(self.o_proj.weight.detach()), f[1], [False, False]]
             if not _recording(f[0]):
                 self._int8 = w
         return w

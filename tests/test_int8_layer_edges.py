@@ -30,6 +30,88 @@ def ring(st):
     return RingPos(int(st.pos), int(st.recent_idx), int(st.recent_filled), None)
 
 
+def fresh_like(mod, kw, dtype):
+    """A new layer with the parameters that ``mod`` has now."""
+    from coda_gqa_l_b200 import CoDAGQALandmarkPerf2
+    new = CoDAGQALandmarkPerf2(**kw).eval().to(dtype).cuda()
+    if mod.o_proj.bias is not None:
+        new.o_proj.bias = torch.nn.Parameter(mod.o_proj.bias.detach().clone())
+    new.load_state_dict(mod.state_dict())
+    new.use_int8_projections = mod.use_int8_projections
+    return new
+
+
+def new_out(mod):
+    n, d, w = mod.num_heads * mod.head_dim, mod.embed_dim, mod.q_proj.weight
+    device, dtype = w.device, w.dtype
+    del mod.o_proj
+    mod.o_proj = torch.nn.Linear(n, d, bias=False, device=device, dtype=dtype)
+
+
+def set_key(mod):
+    mod.k_proj.weight = torch.nn.Parameter(mod.k_proj.weight.detach() * 0.5)
+
+
+def assigned(mod):
+    mod.load_state_dict({k: v * 0.75 if v.is_floating_point() else v.clone() for k, v in mod.state_dict().items()}, assign=True)
+
+
+def add_bias(mod):
+    mod.o_proj.bias = torch.nn.Parameter(torch.ones_like(mod.q_proj.weight[0]))
+
+
+def no_bias(mod):
+    mod.o_proj.bias = None
+
+
+def swapped(mod):
+    """As functional calls do it: past the module's own attribute setting."""
+    mod.v_proj._parameters["weight"] = torch.nn.Parameter(mod.v_proj.weight.detach() * -0.5)
+
+
+CHANGES = (new_out, new_out, set_key, assigned, assigned, swapped, add_bias, no_bias, new_out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kw", SHAPES[:2])
+def test_replaced_parameters_reach_the_prefill(dtype, kw):
+    """A projection deleted and built anew (its memory may come back at the old address), a parameter set, a state dict assigned
+    instead of copied, a bias that comes and goes: the next prefill is that of a fresh layer with the new parameters."""
+    from coda_gqa_l_b200 import _deep_copy_state
+    mod = layer(kw, dtype)
+    x = hidden(2, 30, kw["embed_dim"], dtype, 3)
+    torch.manual_seed(2)
+    s0 = mod.init_state(batch_size=2, device="cuda", dtype=dtype)
+    run = lambda m: m.prefill_chunked(x, _deep_copy_state(s0), block_size=8)[0]  # noqa: E731
+    last = run(mod)
+    for change in CHANGES:
+        with torch.no_grad():
+            change(mod)
+        got = run(mod)
+        assert torch.equal(got, run(fresh_like(mod, kw, dtype))), change.__name__
+        assert not torch.equal(got, last), change.__name__
+        last = got
+
+
+def test_copies_know_another_parameter_at_the_same_address(monkeypatch):
+    """An output weight that lies where the old one lay and counts as many versions: both kinds of derived copies are made again."""
+    mod = on_cpu(monkeypatch)
+    with torch.no_grad():
+        old_t, old_8 = mod._skinny_weights()[2], mod._int8_weights()[2]
+        old = mod.o_proj.weight
+        new = torch.nn.Parameter(old.data)
+        while new._version < old._version:
+            new.mul_(1.0)
+        new.detach().numpy()[...] *= -0.5
+        mod.o_proj.weight = new
+        assert new.data_ptr() == old.data_ptr() and new._version == old._version
+        assert torch.equal(mod._skinny_weights()[2], new.t()) and mod._skinny_weights()[2] is not old_t
+        now = mod._int8_weights()[2]
+        assert now is not old_8 and torch.equal(now.scale, new.abs().amax(1) / 127)
+        again = mod._int8_weights()[2]
+        assert again is now and mod._skinny_weights() is mod._skinny_weights()       # (and not without a reason)
+
+
 def on_cpu(monkeypatch=None):
     """A float32 layer on the CPU, for what the host does with its parameters; rows to 8 bits by their formula."""
     from coda_gqa_l_b200 import CoDAGQALandmarkPerf2, Int8Rows, attention
