@@ -665,32 +665,21 @@ class CoDAGQALandmarkPerf2(nn.Module):
         """Everything an eager decode step needs besides the state, gathered once and re-validated cheaply: the fused
         and transposed weights, the constant tables and their raw addresses.  ``step()`` is called once per layer per
         token by adapter-driven loops, where the host time of walking ``nn.Module`` attributes and rebuilding cache
-        keys (~60 us per call) outweighs the kernels; the bundle is checked by module identity plus address and
-        version counter of every parameter it was built from.  None where the fused layout does not apply."""
+        keys (~60 us per call) outweighs the kernels; the bundle is checked by identity of every module and parameter it
+        was built from, and the parameters' addresses and version counters.  None where the fused layout does not apply."""
         c = self.__dict__.get("_bundle")
-        mods = self._modules
-        if c is not None and c["dev"] == device and c["dt"] == dtype:
-            ok = all(mods[n] is m for n, m in c["mods"])
-            if ok:
-                for prm, ver, ptr in c["stamps"]:
-                    if prm._version != ver or prm.data_ptr() != ptr:
-                        ok = False
-                        break
-            if ok:
-                return c
+        if c is not None and c["dev"] == device and c["dt"] == dtype and self._unchanged(c["mods"], c["stamps"]):
+            return c
         f = self._fused_weight()
         wt = self._skinny_weights()
         if f is None or wt is None or f[0].device != device or f[0].dtype != dtype:
             self.__dict__["_bundle"] = None
             return None
         inv_freq, cos_t, sin_t, eta, nw = self._consts(device, dtype)
-        names = ("q_proj", "k_proj", "v_proj", "lambda_proj", "write_proj", "o_proj", "head_norm", "rope")
-        prms = [p for n in names[:6] for p in mods[n].parameters()] + [self.theta, self.summary_eta_logit, self.rope.inv_freq]
-        if nw is not None:
-            prms.append(self.head_norm.weight)
+        mods, stamps = self._stamps()
         H, Hkv, Dh = self.num_heads, self.num_kv_heads, self.head_dim
         es = f[0].element_size()
-        c = dict(dev=device, dt=dtype, mods=[(n, mods[n]) for n in names], stamps=[(p, p._version, p.data_ptr()) for p in prms],
+        c = dict(dev=device, dt=dtype, mods=mods, stamps=stamps,
                  bias=f[1], w_in_t=wt[1], w_out_t=wt[2], npad=f[0].shape[0], nq=H * Dh, nkv=Hkv * Dh,
                  off_k=H * Dh * es, off_v=(H * Dh + Hkv * Dh) * es, off_lam=(H * Dh + 2 * Hkv * Dh) * es,
                  off_gate=(H * Dh + 2 * Hkv * Dh + H) * es, gated=self.write_policy != "none",
@@ -706,6 +695,29 @@ class CoDAGQALandmarkPerf2(nn.Module):
         if not _recording(f[0]):
             self.__dict__["_bundle"] = c
         return c
+
+    _GATHERED = ("q_proj", "k_proj", "v_proj", "lambda_proj", "write_proj", "o_proj", "head_norm", "rope")
+
+    def _stamps(self):
+        """(modules, parameters) that an eager step's addresses come from, each as (where it is registered, name, what it is
+        now), a parameter with its version counter and address.  A bias that is not there is one, too: it may come."""
+        mods = [(n, self._modules[n]) for n in self._GATHERED]
+        where = [(m._parameters, n) for _, m in mods[:6] for n in ("weight", "bias")]
+        where += [(self._parameters, "theta"), (self._parameters, "summary_eta_logit"), (self.rope._buffers, "inv_freq")]
+        if self.head_norm_mode == "full":
+            where.append((self.head_norm._parameters, "weight"))
+        now = [(d, n, d.get(n)) for d, n in where]
+        return mods, [(d, n, t, 0, 0) if t is None else (d, n, t, t._version, t.data_ptr()) for d, n, t in now]
+
+    def _unchanged(self, mods, stamps) -> bool:
+        have = self._modules
+        for n, m in mods:
+            if have.get(n) is not m:
+                return False
+        for d, n, t, version, ptr in stamps:
+            if d.get(n) is not t or (t is not None and (t._version != version or t.data_ptr() != ptr)):
+                return False
+        return True
 
     def _one_call_ok(self, bd, B: int) -> bool:
         """Whether both projections of a decode step with ``B`` rows run on this library's skinny GEMM with the bundle's
@@ -741,18 +753,13 @@ class CoDAGQALandmarkPerf2(nn.Module):
     def _int8_bundle(self, device, dtype):
         """What :meth:`_decode_bundle` gathers, for a step with 8-bit projections."""
         c = self.__dict__.get("_bundle8")
-        mods = self._modules
-        if (c is not None and c["dev"] == device and c["dt"] == dtype and c["w"] is self._int8 and all(mods[n] is m for n, m in c["mods"])
-                and all(p._version == ver and p.data_ptr() == ptr for p, ver, ptr in c["stamps"])):
+        if c is not None and c["dev"] == device and c["dt"] == dtype and c["w"] is self._int8 and self._unchanged(c["mods"], c["stamps"]):
             return c
         w, f = self._int8_weights(), self._fused_weight()
         if f[0].device != device or f[0].dtype != dtype:
             return None
         inv_freq, cos_t, sin_t, eta, nw = self._consts(device, dtype)
-        names = ("q_proj", "k_proj", "v_proj", "lambda_proj", "write_proj", "o_proj", "head_norm", "rope")
-        prms = [p for n in names[:6] for p in mods[n].parameters()] + [self.theta, self.summary_eta_logit, self.rope.inv_freq]
-        if nw is not None:
-            prms.append(self.head_norm.weight)
+        mods, stamps = self._stamps()
         nq, nkv, es = self.num_heads * self.head_dim, self.num_kv_heads * self.head_dim, f[0].element_size()
         ob = self.o_proj.bias
         layer = StepLayer(bias=f[1].data_ptr(), inv_freq=inv_freq.data_ptr(), eta_logit=eta.data_ptr(), cos_theta=cos_t.data_ptr(),
@@ -762,7 +769,7 @@ class CoDAGQALandmarkPerf2(nn.Module):
         w8 = StepLayerInt8(w_in=w[1][0].data_ptr(), w_in_scale=w[1][1].data_ptr(), w_out=w[2][0].data_ptr(), w_out_scale=w[2][1].data_ptr(),
                            out_bias=_p(ob), w_in_rs=w[1][0].stride(0), w_out_rs=w[2][0].stride(0))
         c = dict(
-            dev=device, dt=dtype, w=w, mods=[(n, mods[n]) for n in names], stamps=[(p, p._version, p.data_ptr()) for p in prms],
+            dev=device, dt=dtype, w=w, mods=mods, stamps=stamps,
             layer=layer, w8=w8, layer_ptr=C.addressof(layer), w8_ptr=C.addressof(w8), ws={}, n_out=layer.n_out,
             keep=(inv_freq, cos_t, sin_t, eta, nw, f, ob))
         if not _recording(f[0]):

@@ -198,3 +198,62 @@ def test_first_call_captured_then_replayed_beside_calls_outside(int8):
         same(got, want)
         assert torch.equal(run(mod, _deep_copy_state(s0)), want)
     assert mod.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("int8", [True, False])
+def test_replaced_parameters_reach_the_eager_step(int8):
+    """The same for the eager step alone, which runs from addresses gathered once."""
+    from coda_gqa_l_b200 import _deep_copy_state
+    dtype, kw = SHAPES[1]
+    mod = layer(kw, dtype, int8=int8)
+    x = hidden(2, 4, kw["embed_dim"], dtype, 3)
+    torch.manual_seed(2)
+    s0 = mod.init_state(batch_size=2, device="cuda", dtype=dtype)
+
+    def run(m):
+        s = _deep_copy_state(s0)
+        return torch.cat([m.step(x[:, t:t + 1].contiguous(), s)[0] for t in range(4)], dim=1)
+
+    last = run(mod)
+    for change in CHANGES:
+        with torch.no_grad():
+            change(mod)
+        got = run(mod)
+        assert torch.equal(got, run(fresh_like(mod, kw, dtype))), change.__name__
+        assert not torch.equal(got, last), change.__name__
+        last = got
+
+
+@pytest.mark.parametrize("int8", [True, False])
+def test_gathered_addresses_know_replaced_parameters(int8, monkeypatch):
+    """Each way to replace a parameter makes the eager step gather its addresses again, and nothing else does."""
+    mod = on_cpu(monkeypatch)
+    mod.use_int8_projections = int8
+    gather = lambda: (mod._int8_bundle if int8 else mod._decode_bundle)(torch.device("cpu"), torch.float32)  # noqa: E731
+    with torch.no_grad():
+        last = gather()
+        assert gather() is last
+        for change in CHANGES:
+            if change is add_bias and not int8:
+                break                                  # (gathered without one only)
+            change(mod)
+            now = gather()
+            assert now is not last, change.__name__
+            f = mod._fused_weight()
+            assert now["layer"].bias == f[1].data_ptr()
+            if int8:
+                assert now["w8"].out_bias == (None if mod.o_proj.bias is None else mod.o_proj.bias.data_ptr())
+                assert now["w8"].w_in == mod._int8_weights()[1].values.data_ptr()
+            else:
+                assert now["w_in"] == f[0].data_ptr() and now["w_out"] == mod.o_proj.weight.data_ptr()
+            assert gather() is now
+            last = now
+        if not int8:
+            add_bias(mod)
+            assert gather() is None
+            no_bias(mod)
+            assert gather() is not None
+        mod.rope.inv_freq = mod.rope.inv_freq * 0.5
+        now = gather()
+        assert now is not last and now["layer"].inv_freq == mod._consts(torch.device("cpu"), torch.float32)[0].data_ptr()
