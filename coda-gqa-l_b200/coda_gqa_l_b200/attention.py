@@ -755,13 +755,14 @@ class CoDAGQALandmarkPerf2(nn.Module):
         c = self.__dict__.get("_bundle8")
         if c is not None and c["dev"] == device and c["dt"] == dtype and c["w"] is self._int8 and self._unchanged(c["mods"], c["stamps"]):
             return c
-        w, f = self._int8_weights(), self._fused_weight()
+        w, f, ob = self._int8_weights(), self._fused_weight(), self.o_proj.bias
         if f[0].device != device or f[0].dtype != dtype:
             return None
+        if ob is not None and not (ob.device == device and ob.dtype == dtype and ob.is_contiguous()):
+            return None                                    # (read as it lies, in the state's type)
         inv_freq, cos_t, sin_t, eta, nw = self._consts(device, dtype)
         mods, stamps = self._stamps()
         nq, nkv, es = self.num_heads * self.head_dim, self.num_kv_heads * self.head_dim, f[0].element_size()
-        ob = self.o_proj.bias
         layer = StepLayer(bias=f[1].data_ptr(), inv_freq=inv_freq.data_ptr(), eta_logit=eta.data_ptr(), cos_theta=cos_t.data_ptr(),
                           sin_theta=sin_t.data_ptr(), norm_w=_p(nw), embed=self.embed_dim, npad=f[0].shape[0], n_heads_out=nq,
                           n_out=self.o_proj.weight.shape[0], off_k=nq * es, off_v=(nq + nkv) * es, off_lam=(nq + 2 * nkv) * es,

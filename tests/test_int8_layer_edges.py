@@ -257,3 +257,17 @@ def test_gathered_addresses_know_replaced_parameters(int8, monkeypatch):
         mod.rope.inv_freq = mod.rope.inv_freq * 0.5
         now = gather()
         assert now is not last and now["layer"].inv_freq == mod._consts(torch.device("cpu"), torch.float32)[0].data_ptr()
+
+
+def test_output_bias_of_another_type_takes_the_general_path(monkeypatch):
+    """The native step reads the bias in the state's type: it does not take a layer whose output bias has another."""
+    mod = on_cpu(monkeypatch)
+    mod.use_int8_projections = True
+    with torch.no_grad():
+        add_bias(mod)
+        mod.o_proj.bias = torch.nn.Parameter(mod.o_proj.bias.detach().bfloat16())
+        assert mod._int8_bundle(torch.device("cpu"), torch.float32) is None
+        mod.o_proj.bias = torch.nn.Parameter(torch.ones(2 * mod.embed_dim)[::2])
+        assert mod._int8_bundle(torch.device("cpu"), torch.float32) is None
+        add_bias(mod)
+        assert mod._int8_bundle(torch.device("cpu"), torch.float32) is not None
