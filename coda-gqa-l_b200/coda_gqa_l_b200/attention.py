@@ -74,6 +74,13 @@ def _recording(t: torch.Tensor) -> bool:
     return t.is_cuda and torch.cuda.is_current_stream_capturing()
 
 
+def _settle(t: torch.Tensor) -> None:
+    """The host waits for what was just made on ``t``'s current stream: copies derived from the parameters are made once, by
+    whichever call comes first, and serve calls on every stream from then on, with no event to tell those of it."""
+    if t.is_cuda and torch._C._len_torch_dispatch_stack() == 0:
+        torch.cuda.current_stream(t.device).synchronize()
+
+
 def _p(t: Optional[torch.Tensor]) -> Optional[int]:
     return None if t is None else t.data_ptr()
 
@@ -228,7 +235,7 @@ class CoDAGQALandmarkPerf2(nn.Module):
         # of the rounded weights and inputs.  Inputs may then come in 8 bits already (Int8Rows from add_rms_norm).
         # Keeps the 8-bit copies beside the parameters; they follow the parameters as the other derived copies do.
         self.use_int8_projections = False
-        self._int8 = None
+        self._int8 = self._int8_rows = None
         self._gemm_ok: Dict[tuple, bool] = {}
         # Second half of a split decode step (after route_launch / the stack's batched routing) as one launch:
         # the attention kernel writes the new token itself (coda_b200_decode_attend_append).
@@ -482,6 +489,7 @@ class CoDAGQALandmarkPerf2(nn.Module):
                 self.summary_eta_logit.detach().to(device=device, dtype=torch.float32).contiguous(),
                 None if nw is None else nw.detach().to(device=device, dtype=dtype).contiguous())
         if not _recording(th):
+            _settle(th)
             self._const_cache["k"] = (key, vals)
         return vals
 
@@ -525,6 +533,7 @@ class CoDAGQALandmarkPerf2(nn.Module):
             off += l.out_features
         if recording:
             return W, b
+        _settle(W)
         self._fused = (W, b)
         self._fused_ptrs = [(l.weight.data_ptr(), None if l.bias is None else l.bias.data_ptr()) for l in lins]
         return self._fused
@@ -546,6 +555,7 @@ class CoDAGQALandmarkPerf2(nn.Module):
         if wt is None or not self._made_from(wt[0], f):
             wt = (self._sources(f), f[0].t().contiguous(), self.o_proj.weight.detach().t().contiguous())
             if not _recording(f[0]):
+                _settle(f[0])
                 self._wt = wt
         return wt
 
@@ -573,25 +583,35 @@ class CoDAGQALandmarkPerf2(nn.Module):
         self._int8 = None
 
     def _int8_weights(self):
-        """[sources, fused input weight and output weight in 8 bits, fused bias, used]: quantised on first use and again when a
-        parameter is another tensor or its version counter moves.  ``used``: which of the two has been through a product since, so
-        that the next one may request it ahead of its turn (int8_gemm's ``w_ready``)."""
+        """(sources, fused input weight and output weight in 8 bits, fused bias, ready): quantised on first use and again when a
+        parameter is another tensor or its version counter moves, into the same memory then, once no stream reads it any
+        more: a graph that was captured around the layer goes on with the new values.  ``ready``: complete before anything
+        that is launched from now on (int8_gemm's ``w_ready``)."""
         f = self._fused_weight()
         if f is None or type(self.o_proj) is not nn.Linear:
             raise RuntimeError("use_int8_projections needs plain nn.Linear projections")
         w = self._int8
         if w is None or not self._made_from(w[0], f):
-            w = [self._sources(f), quantize_int8(f[0]), quantize_int8(self.o_proj.weight.detach()), f[1], [False, False]]
-            if not _recording(f[0]):
-                self._int8 = w
+            sources, rows = self._sources(f), (quantize_int8(f[0]), quantize_int8(self.o_proj.weight.detach()))
+            if _recording(f[0]):
+                return (sources, *rows, f[1], False)
+            old = self._int8_rows
+            if old is not None and all(a.values.shape == b.values.shape and a.values.device == b.values.device for a, b in zip(old, rows)):
+                if f[0].is_cuda:
+                    torch.cuda.synchronize(f[0].device)
+                for a, b in zip(old, rows):
+                    a.values.copy_(b.values)
+                    a.scale.copy_(b.scale)
+                rows = tuple(Int8Rows(*a) for a in old)
+            _settle(f[0])
+            self._int8_rows = rows
+            w = self._int8 = (sources, *rows, f[1], True)
         return w
 
     def _int8_product(self, rows: Int8Rows, which: int, bias, residual, dtype) -> torch.Tensor:
         """``rows`` through the input (0) or output (1) projection's 8-bit weight."""
         w = self._int8_weights()
-        y = int8_gemm(rows, w[1 + which], bias, residual, dtype, self._status_word(rows[0].device), w_ready=w[4][which])
-        w[4][which] = True
-        return y
+        return int8_gemm(rows, w[1 + which], bias, residual, dtype, self._status_word(rows[0].device), w_ready=w[4])
 
     def _gemm_workspace(self, device, nbytes: int) -> torch.Tensor:
         """Split-K workspace of coda_b200_proj_gemm: one per device for every layer of the process (the calls of a
@@ -804,14 +824,13 @@ class CoDAGQALandmarkPerf2(nn.Module):
             n = bd["ws"][B] = int(lib.coda_b200_step_layer_int8_ws_bytes(bd["layer_ptr"], B))
         ws = torch.empty(n, device=dev, dtype=torch.uint8)
         y = torch.empty((B, 1, bd["n_out"]), device=dev, dtype=dt)
-        used = bd["w"][4]
+        ready = bd["w"][4]
         rc = lib.coda_b200_step_layer_int8(
             bd["layer_ptr"], bd["w8_ptr"], C.addressof(cfg), C.addressof(ptrs), RingPos(st.pos, st.recent_idx, st.recent_filled, None),
             None if in8 else t.data_ptr(), t.data_ptr() if in8 else None, t.stride(0) if in8 else 0, x.scale.data_ptr() if in8 else None,
-            _p(residual), used[0], used[1], ws.data_ptr(), y.data_ptr(), self._decode_records(cfg, dev).data_ptr(),
+            _p(residual), ready, ready, ws.data_ptr(), y.data_ptr(), self._decode_records(cfg, dev).data_ptr(),
             self._status_word(dev).data_ptr(), _stream(dev))
         if rc == 0 or rc <= _lib.CODA_CACHE_WRITTEN:          # (the token is in the ring, whatever came after)
-            used[0] = used[1] = True
             self.advance_host_scalars(st)
         if rc:
             check(rc, "coda_b200_step_layer_int8")

@@ -147,5 +147,6 @@ def int8_linear(x: Int8Rows, weight: Int8Rows, bias: Optional[torch.Tensor] = No
 def int8_gemm(x: Int8Rows, weight: Int8Rows, bias: Optional[torch.Tensor], residual: Optional[torch.Tensor], dtype: torch.dtype,
               status: Optional[torch.Tensor], w_ready: bool = False) -> torch.Tensor:
     """:func:`int8_linear` for a caller with a status word of its own.  ``w_ready``: the weight's values were complete
-    before an earlier product on this stream began, so they may be requested while the kernels ahead of this one still run."""
+    before this call, or before an earlier product on this stream began, so they may be requested while the kernels ahead
+    of this one still run."""
     return _calls().int8_linear(x[0], x[1], weight[0], weight[1], bias, residual, dtype, status, w_ready)

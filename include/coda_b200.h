@@ -460,8 +460,8 @@ int coda_b200_dequantize_rows(int32_t dtype, int64_t rows, int32_t dim, const in
  * (an nn.Linear weight's layout), the sum exact in 32-bit integers (K <= 131071), the rest fp32, rounded once to `dtype`,
  * the type of y, bias and residual.  Rows of x and w start on 16-byte boundaries (row strides in bytes, multiples of 16;
  * what lies behind K in a row is not read into the sum).  residual may be y itself.  w_ready != 0: the values of w were
- * complete before an earlier product on this stream began (weights quantised once, from their second use on), so a
- * kernel for few tokens may request them while the kernels ahead of it still run.  status: optional device int, set non-zero if a bounded wait expired. */
+ * complete before this call was made, or before an earlier product on this stream began; the kernel may then request them
+ * while the kernels ahead of it still run.  status: optional device int, set non-zero if a bounded wait expired. */
 int coda_b200_int8_gemm(int32_t dtype, int32_t M, int32_t K, int32_t N, const int8_t* x, int64_t x_rs, const float* x_scale,
                         const int8_t* w, int64_t w_rs, const float* w_scale, const void* bias,
                         const void* residual, int64_t res_rs, void* y, int64_t y_rs, int32_t w_ready, int32_t* status,

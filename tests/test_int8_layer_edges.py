@@ -271,3 +271,96 @@ def test_output_bias_of_another_type_takes_the_general_path(monkeypatch):
         assert mod._int8_bundle(torch.device("cpu"), torch.float32) is None
         add_bias(mod)
         assert mod._int8_bundle(torch.device("cpu"), torch.float32) is not None
+
+
+def test_copies_are_made_again_into_the_same_memory(monkeypatch):
+    """A graph captured around a layer holds the addresses of its 8-bit copies: they stay when the parameters change."""
+    from coda_gqa_l_b200 import attention
+    mod = on_cpu(monkeypatch)
+    with torch.no_grad():
+        a = mod._int8_weights()
+        where = [t.data_ptr() for r in a[1:3] for t in r]
+        for change in (lambda: mod.k_proj.weight.mul_(0.5), lambda: new_out(mod), lambda: assigned(mod),
+                       lambda: (mod.o_proj.weight.data.mul_(3.0), mod.refresh_weights())):
+            change()
+            b = mod._int8_weights()
+            assert b is not a and [t.data_ptr() for r in b[1:3] for t in r] == where
+            for r, w in ((b[1], mod._fused_weight()[0]), (b[2], mod.o_proj.weight)):
+                want = attention.quantize_int8(w.detach())
+                assert torch.equal(r.values, want.values) and torch.equal(r.scale, want.scale)
+            a = b
+
+
+@pytest.mark.gpu
+def test_two_streams_share_a_layer_that_neither_has_used():
+    """The first call of a layer on one stream, held up there, and the second on another with no event between them; then a
+    call held up on the second stream while the first changes the weights: each result is that of the weights at its call."""
+    from coda_gqa_l_b200 import _deep_copy_state
+    dtype, kw = SHAPES[1]
+    x = hidden(2, 64, kw["embed_dim"], dtype, 3)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    for trial in range(4):
+        mod, ref = layer(kw, dtype, seed=trial), layer(kw, dtype, seed=trial)
+        torch.manual_seed(trial)
+        s0 = mod.init_state(batch_size=2, device="cuda", dtype=dtype)
+        states = [_deep_copy_state(s0) for _ in range(6)]
+        run = lambda m, s: m.prefill_chunked(x, s, block_size=32)[0]  # noqa: E731
+        want = run(ref, states[0])
+        torch.cuda.synchronize()
+        with torch.cuda.stream(a):
+            torch.cuda._sleep(4_000_000)                       # some 2 ms
+            ya = run(mod, states[1])
+        with torch.cuda.stream(b):
+            yb = run(mod, states[2])
+        torch.cuda.synchronize()
+        assert torch.equal(ya, want) and torch.equal(yb, want)
+        with torch.cuda.stream(b):
+            torch.cuda._sleep(4_000_000)
+            yb = run(mod, states[3])
+        with torch.cuda.stream(a), torch.no_grad():
+            mod.q_proj.weight.mul_(-1.0)
+            mod.o_proj.weight.mul_(0.5)
+            ya = run(mod, states[4])
+        torch.cuda.synchronize()
+        assert torch.equal(yb, want)
+        with torch.no_grad():
+            ref.q_proj.weight.mul_(-1.0)
+            ref.o_proj.weight.mul_(0.5)
+        assert torch.equal(ya, run(ref, states[5])) and not torch.equal(ya, want)
+
+
+@pytest.mark.gpu
+def test_graph_captured_by_hand_follows_changed_weights():
+    """A replay of a graph around a layer's prefill after its weights changed, the old copies' memory having been offered to
+    others: the results of the new weights once a call outside has taken them over, of the old ones before."""
+    from coda_gqa_l_b200 import _deep_copy_state
+    dtype, kw = SHAPES[1]
+    mod = layer(kw, dtype)
+    x = hidden(2, 40, kw["embed_dim"], dtype, 3)
+    torch.manual_seed(2)
+    s0 = mod.init_state(batch_size=2, device="cuda", dtype=dtype)
+    run = lambda s: mod.prefill_chunked(x, s, block_size=16)[0]  # noqa: E731
+    first = run(_deep_copy_state(s0))
+    s1 = _deep_copy_state(s0)
+    arena = s1._arena.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(s1)
+
+    def replayed():
+        s1._arena.copy_(arena)
+        graph.replay()
+        torch.cuda.synchronize()
+        return got.clone()
+
+    assert torch.equal(replayed(), first)
+    with torch.no_grad():
+        for p in (mod.k_proj.weight, mod.o_proj.weight):
+            p.mul_(-0.7)
+    assert torch.equal(replayed(), first)
+    second = run(_deep_copy_state(s0))
+    junk = [torch.full((n,), 77, device="cuda", dtype=torch.int8) for n in (mod._int8[1].values.numel(), mod._int8[2].values.numel()) for _ in range(4)]
+    assert torch.equal(replayed(), second) and not torch.equal(second, first)
+    mod.refresh_weights()
+    junk += [torch.full_like(junk[0], 77) for _ in range(4)]
+    assert torch.equal(run(_deep_copy_state(s0)), second) and torch.equal(replayed(), second)
