@@ -203,7 +203,7 @@ class CoDAGQALandmarkPerf2(nn.Module):
 
         self._cfg_cache: Dict[tuple, LayerCfg] = {}
         self._const_cache: Dict[tuple, tuple] = {}
-        self._scratch: Dict[tuple, torch.Tensor] = {}
+        self._scratch: Dict[tuple, Tuple[int, torch.Tensor]] = {}
         self._fused = None
         self._fused_ptrs = []
         self._wt = None
@@ -726,17 +726,20 @@ class CoDAGQALandmarkPerf2(nn.Module):
         where += [(self._parameters, "theta"), (self._parameters, "summary_eta_logit"), (self.rope._buffers, "inv_freq")]
         if self.head_norm_mode == "full":
             where.append((self.head_norm._parameters, "weight"))
-        now = [(d, n, d.get(n)) for d, n in where]
+        now = [(d, n, d[n]) for d, n in where]
         return mods, [(d, n, t, 0, 0) if t is None else (d, n, t, t._version, t.data_ptr()) for d, n, t in now]
 
     def _unchanged(self, mods, stamps) -> bool:
         have = self._modules
-        for n, m in mods:
-            if have.get(n) is not m:
-                return False
-        for d, n, t, version, ptr in stamps:
-            if d.get(n) is not t or (t is not None and (t._version != version or t.data_ptr() != ptr)):
-                return False
+        try:
+            for n, m in mods:
+                if have[n] is not m:
+                    return False
+            for d, n, t, version, ptr in stamps:
+                if d[n] is not t or (t is not None and (t._version != version or t.data_ptr() != ptr)):
+                    return False
+        except KeyError:                       # (one was deleted)
+            return False
         return True
 
     def _one_call_ok(self, bd, B: int) -> bool:
@@ -824,12 +827,12 @@ class CoDAGQALandmarkPerf2(nn.Module):
             n = bd["ws"][B] = int(lib.coda_b200_step_layer_int8_ws_bytes(bd["layer_ptr"], B))
         ws = torch.empty(n, device=dev, dtype=torch.uint8)
         y = torch.empty((B, 1, bd["n_out"]), device=dev, dtype=dt)
-        ready = bd["w"][4]
+        ready, stream = bd["w"][4], _stream(dev)
         rc = lib.coda_b200_step_layer_int8(
             bd["layer_ptr"], bd["w8_ptr"], C.addressof(cfg), C.addressof(ptrs), RingPos(st.pos, st.recent_idx, st.recent_filled, None),
             None if in8 else t.data_ptr(), t.data_ptr() if in8 else None, t.stride(0) if in8 else 0, x.scale.data_ptr() if in8 else None,
-            _p(residual), ready, ready, ws.data_ptr(), y.data_ptr(), self._decode_records(cfg, dev).data_ptr(),
-            self._status_word(dev).data_ptr(), _stream(dev))
+            _p(residual), ready, ready, ws.data_ptr(), y.data_ptr(), self._decode_records(cfg, dev, stream).data_ptr(),
+            self._status_word(dev).data_ptr(), stream)
         if rc == 0 or rc <= _lib.CODA_CACHE_WRITTEN:          # (the token is in the ring, whatever came after)
             self.advance_host_scalars(st)
         if rc:
@@ -868,10 +871,11 @@ class CoDAGQALandmarkPerf2(nn.Module):
                 # one workspace (projection rows, then head outputs) and one native call for the step's four launches
                 ws = torch.empty(B * (bd["npad"] + bd["nq"]), device=dev, dtype=x.dtype)
                 y = torch.empty((B, 1, bd["n_out"]), device=dev, dtype=x.dtype)
+                s = _stream(dev)
                 rc = lib.coda_b200_step_layer(bd["layer_ptr"], C.addressof(cfg), C.addressof(ptrs),
                                               RingPos(st.pos, st.recent_idx, st.recent_filled, None), xp, rp_ or None,
-                                              ws.data_ptr(), y.data_ptr(), self._decode_records(cfg, dev).data_ptr(),
-                                              self._status_word(dev).data_ptr(), _stream(dev))
+                                              ws.data_ptr(), y.data_ptr(), self._decode_records(cfg, dev, s).data_ptr(),
+                                              self._status_word(dev).data_ptr(), s)
                 if rc == 0 or rc <= _lib.CODA_CACHE_WRITTEN:      # (the token is in the ring, whatever came after)
                     self.advance_host_scalars(st)
                 if rc:
@@ -898,7 +902,7 @@ class CoDAGQALandmarkPerf2(nn.Module):
             return None
         s = _stream(dev)
         rp = RingPos(st.pos, st.recent_idx, st.recent_filled, None)
-        qrec = self._decode_records(cfg, dev)
+        qrec = self._decode_records(cfg, dev, s)
         out = torch.empty((B, self.num_heads * self.head_dim), device=dev, dtype=x.dtype)
         status = self._status_word(dev).data_ptr()
         gate = base + bd["off_gate"] if bd["gated"] else None
@@ -1101,16 +1105,26 @@ class CoDAGQALandmarkPerf2(nn.Module):
         (1 = producer waiting for a free tile, 2 = consumer waiting for a tile).  Synchronises."""
         return 0 if self._status is None else int(self._status.item())
 
-    def _decode_records(self, cfg, device) -> torch.Tensor:
-        """Device buffer for the per-plane decode records (prepared queries, lambda, visibility mask)."""
+    def _decode_records(self, cfg, device, stream: Optional[int] = None) -> torch.Tensor:
+        """Device buffer for the per-plane decode records (prepared queries, lambda, visibility mask): one for each stream
+        that calls the layer, and one of its own for a call that is captured into a graph."""
         n = getattr(cfg, "_rec_bytes", None)
         if n is None:
             n = int(lib.coda_b200_decode_record_bytes(C.byref(cfg)))
             cfg._rec_bytes = n
-        buf = self._qrec
-        if buf is None or buf.numel() < n or buf.device != device:
-            buf = torch.empty(n, dtype=torch.uint8, device=device)
-            self._qrec = buf
+        buf = self.__dict__["_qrec"] = self._workspace("records", n, device, _stream(device) if stream is None else stream)
+        return buf
+
+    def _workspace(self, what: str, n: int, device, stream: int) -> torch.Tensor:
+        """``n`` bytes or more for what a call writes and reads again: calls on one stream follow one another, so they share
+        it; calls on two streams, or replays of two graphs, may run side by side."""
+        key = (what, device.index, stream)
+        kept = self._scratch.get(key)
+        if kept is not None and kept[0] >= n:
+            return kept[1]
+        buf = torch.empty(n, dtype=torch.uint8, device=device)
+        if not _recording(buf):
+            self._scratch[key] = (n, buf)
         return buf
 
     def _fused_write_ok(self, cfg, q: Optional[torch.Tensor] = None) -> bool:
@@ -1261,7 +1275,7 @@ class CoDAGQALandmarkPerf2(nn.Module):
         _, _, _, _, nw = self._consts(out.device, out.dtype)
         ptrs = self._ptrs(state)
         check(lib.coda_b200_decode_attend_prepared(
-            C.byref(cfg), C.byref(ptrs), self._decode_records(cfg, out.device).data_ptr(), _p(nw), out.data_ptr(),
+            C.byref(cfg), C.byref(ptrs), self._qrec.data_ptr(), _p(nw), out.data_ptr(),
             out.stride(0), self._status_word(out.device).data_ptr(), _stream()), "coda_b200_decode_attend_prepared")
 
     def step_graphable(self, x: torch.Tensor, state: CoDAGQALandmarkStatePerf2, rp: RingPos,
@@ -1432,13 +1446,7 @@ class CoDAGQALandmarkPerf2(nn.Module):
         st.recent_idx = 0
 
     def _route_scratch(self, cfg, device) -> torch.Tensor:
-        n = int(lib.coda_b200_route_scratch_bytes(C.byref(cfg)))
-        key = (device, n)
-        t = self._scratch.get(key)
-        if t is None:
-            t = torch.empty(n, dtype=torch.uint8, device=device)
-            self._scratch[key] = t
-        return t
+        return self._workspace("routing", int(lib.coda_b200_route_scratch_bytes(C.byref(cfg))), device, _stream(device))
 
     @torch.no_grad()
     def prefill_chunked(self, x_seq: torch.Tensor, state: CoDAGQALandmarkStatePerf2, *, block_size: int = 256,

@@ -364,3 +364,60 @@ def test_graph_captured_by_hand_follows_changed_weights():
     mod.refresh_weights()
     junk += [torch.full_like(junk[0], 77) for _ in range(4)]
     assert torch.equal(run(_deep_copy_state(s0)), second) and torch.equal(replayed(), second)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("int8", [True, False])
+def test_two_streams_and_two_graphs_share_a_layer(int8):
+    """Prefills that evict and steps of one layer on two streams side by side, each with states of its own, then two graphs of
+    a step replayed side by side: the results of one after the other."""
+    from coda_gqa_l_b200 import _deep_copy_state
+    dtype, kw = SHAPES[1]
+    mod = layer(kw, dtype, int8=int8)
+    xs = [hidden(8, 300, kw["embed_dim"], dtype, i) for i in range(2)]
+    torch.manual_seed(2)
+    first = [mod.init_state(batch_size=8, device="cuda", dtype=dtype) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+
+    def run(x, s):
+        out = [mod.prefill_chunked(x[:, :280], s, block_size=40)[0]]
+        return out + [mod.step(x[:, t:t + 1].contiguous(), s)[0] for t in range(280, 300)]
+
+    def side_by_side(calls):
+        torch.cuda.synchronize()
+        for st in streams:
+            with torch.cuda.stream(st):
+                torch.cuda._sleep(2_000_000)
+        out = []
+        for st, call in zip(streams, calls):
+            with torch.cuda.stream(st):
+                out.append(call())
+        torch.cuda.synchronize()
+        return out
+
+    ends = [_deep_copy_state(s) for s in first]
+    want = [run(x, s) for x, s in zip(xs, ends)]
+    for _ in range(4):
+        states = [_deep_copy_state(s) for s in first]
+        got = side_by_side([lambda x=x, s=s: run(x, s) for x, s in zip(xs, states)])
+        for a, b, p, q in zip(got, want, states, ends):
+            assert all(torch.equal(u, v) for u, v in zip(a, b))
+            assert all(torch.equal(getattr(p, f), getattr(q, f)) for f in FIELDS)
+    graphs = []
+    for x, s in zip(xs, ends):
+        xt = x[:, :1].contiguous()
+        g = torch.cuda.CUDAGraph()
+        arena = s._arena.clone()
+        with torch.cuda.graph(g):
+            y = mod.step(xt, s)[0]
+        g.replay()
+        torch.cuda.synchronize()
+        graphs.append((g, y, y.clone(), s, arena, s._arena.clone(), xt))
+    for _ in range(10):
+        for g, y, ref, s, arena, after, xt in graphs:
+            s._arena.copy_(arena)
+            y.zero_()
+        side_by_side([e[0].replay for e in graphs])
+        for g, y, ref, s, arena, after, xt in graphs:
+            assert torch.equal(y, ref) and torch.equal(s._arena, after)
+    assert mod.device_status() == 0
