@@ -582,19 +582,21 @@ class CoDAGQALandmarkPerf2(nn.Module):
         self._wt = None
         self._int8 = None
 
-    def _int8_weights(self):
-        """(sources, fused input weight and output weight in 8 bits, fused bias, ready): quantised on first use and again when a
+    def _int8_weights(self, f=None):
+        """(sources, fused input weight and output weight in 8 bits, fused bias): quantised on first use and again when a
         parameter is another tensor or its version counter moves, into the same memory then, once no stream reads it any
-        more: a graph that was captured around the layer goes on with the new values.  ``ready``: complete before anything
-        that is launched from now on (int8_gemm's ``w_ready``)."""
-        f = self._fused_weight()
+        more: a graph that was captured around the layer goes on with the new values.  None where that would fall into a
+        graph capture.  ``f``: :meth:`_fused_weight`, if it is at hand."""
+        if self._int8 is None and _recording(self.theta):
+            return None
+        f = self._fused_weight() if f is None else f
         if f is None or type(self.o_proj) is not nn.Linear:
             raise RuntimeError("use_int8_projections needs plain nn.Linear projections")
         w = self._int8
         if w is None or not self._made_from(w[0], f):
-            sources, rows = self._sources(f), (quantize_int8(f[0]), quantize_int8(self.o_proj.weight.detach()))
             if _recording(f[0]):
-                return (sources, *rows, f[1], False)
+                return None
+            sources, rows = self._sources(f), (quantize_int8(f[0]), quantize_int8(self.o_proj.weight.detach()))
             old = self._int8_rows
             if old is not None and all(a.values.shape == b.values.shape and a.values.device == b.values.device for a, b in zip(old, rows)):
                 if f[0].is_cuda:
@@ -605,13 +607,15 @@ class CoDAGQALandmarkPerf2(nn.Module):
                 rows = tuple(Int8Rows(*a) for a in old)
             _settle(f[0])
             self._int8_rows = rows
-            w = self._int8 = (sources, *rows, f[1], True)
+            w = self._int8 = (sources, *rows, f[1])
         return w
 
-    def _int8_product(self, rows: Int8Rows, which: int, bias, residual, dtype) -> torch.Tensor:
-        """``rows`` through the input (0) or output (1) projection's 8-bit weight."""
-        w = self._int8_weights()
-        return int8_gemm(rows, w[1 + which], bias, residual, dtype, self._status_word(rows[0].device), w_ready=w[4])
+    def _int8_product(self, rows: Int8Rows, which: int, bias, residual, dtype, f=None) -> torch.Tensor:
+        """``rows`` through the input (0) or output (1) projection's 8-bit weight (in a capture without one: a weight that each
+        replay quantises for itself)."""
+        w = self._int8_weights(f)
+        weight = quantize_int8(self.o_proj.weight.detach() if which else f[0]) if w is None else w[1 + which]
+        return int8_gemm(rows, weight, bias, residual, dtype, self._status_word(rows[0].device), w_ready=w is not None)
 
     def _gemm_workspace(self, device, nbytes: int) -> torch.Tensor:
         """Split-K workspace of coda_b200_proj_gemm: one per device for every layer of the process (the calls of a
@@ -778,7 +782,10 @@ class CoDAGQALandmarkPerf2(nn.Module):
         c = self.__dict__.get("_bundle8")
         if c is not None and c["dev"] == device and c["dt"] == dtype and c["w"] is self._int8 and self._unchanged(c["mods"], c["stamps"]):
             return c
-        w, f, ob = self._int8_weights(), self._fused_weight(), self.o_proj.bias
+        w = self._int8_weights()
+        if w is None:
+            return None
+        f, ob = self._fused_weight(), self.o_proj.bias
         if f[0].device != device or f[0].dtype != dtype:
             return None
         if ob is not None and not (ob.device == device and ob.dtype == dtype and ob.is_contiguous()):
@@ -827,11 +834,11 @@ class CoDAGQALandmarkPerf2(nn.Module):
             n = bd["ws"][B] = int(lib.coda_b200_step_layer_int8_ws_bytes(bd["layer_ptr"], B))
         ws = torch.empty(n, device=dev, dtype=torch.uint8)
         y = torch.empty((B, 1, bd["n_out"]), device=dev, dtype=dt)
-        ready, stream = bd["w"][4], _stream(dev)
+        stream = _stream(dev)
         rc = lib.coda_b200_step_layer_int8(
             bd["layer_ptr"], bd["w8_ptr"], C.addressof(cfg), C.addressof(ptrs), RingPos(st.pos, st.recent_idx, st.recent_filled, None),
             None if in8 else t.data_ptr(), t.data_ptr() if in8 else None, t.stride(0) if in8 else 0, x.scale.data_ptr() if in8 else None,
-            _p(residual), ready, ready, ws.data_ptr(), y.data_ptr(), self._decode_records(cfg, dev, stream).data_ptr(),
+            _p(residual), 1, 1, ws.data_ptr(), y.data_ptr(), self._decode_records(cfg, dev, stream).data_ptr(),
             self._status_word(dev).data_ptr(), stream)
         if rc == 0 or rc <= _lib.CODA_CACHE_WRITTEN:          # (the token is in the ring, whatever came after)
             self.advance_host_scalars(st)
@@ -936,11 +943,14 @@ class CoDAGQALandmarkPerf2(nn.Module):
     def _project(self, x: torch.Tensor, need_kv: bool):
         """q, k, v, lambda logits, gate logits as (B, L, features) tensors (upstream attention.py:396-410,508)."""
         if self.use_int8_projections:
-            bias = self._int8_weights()[3]
+            f = self._fused_weight()
+            if f is None or type(self.o_proj) is not nn.Linear:
+                raise RuntimeError("use_int8_projections needs plain nn.Linear projections")
+            bias = f[1]
             if not isinstance(x, Int8Rows) and x.dtype != bias.dtype:
                 raise RuntimeError(f"input is {x.dtype}, the projections are {bias.dtype}")
             rows = x if isinstance(x, Int8Rows) else quantize_int8(x)
-            q, k, v, lam, gate = self._split_fused(self._int8_product(rows, 0, bias, None, bias.dtype))
+            q, k, v, lam, gate = self._split_fused(self._int8_product(rows, 0, bias, None, bias.dtype, f))
             return (q, k, v, lam, gate) if need_kv else (q, None, None, lam, None)
         f = self._fused_weight() if need_kv else None
         if f is not None:

@@ -421,3 +421,25 @@ def test_two_streams_and_two_graphs_share_a_layer(int8):
         for g, y, ref, s, arena, after, xt in graphs:
             assert torch.equal(y, ref) and torch.equal(s._arena, after)
     assert mod.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_a_capture_without_copies_quantises_each_weight_once(monkeypatch):
+    """A first call inside a capture puts into the graph one quantisation of each weight for each time it is used."""
+    from coda_gqa_l_b200 import attention
+    dtype, kw = SHAPES[1]
+    mod = layer(kw, dtype)
+    x = hidden(2, 20, kw["embed_dim"], dtype, 3)
+    torch.manual_seed(2)
+    s = mod.init_state(batch_size=2, device="cuda", dtype=dtype)
+    rows = []
+    inner = attention.quantize_int8
+    monkeypatch.setattr(attention, "quantize_int8", lambda t: rows.append(t.shape) or inner(t))
+    heads = mod.num_heads * mod.head_dim
+    weights = [(mod.embed_dim, heads)]
+    for call in (lambda: mod.prefill_chunked(x, s, block_size=32), lambda: mod.step(x[:, :1].contiguous(), s)):
+        rows.clear()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call()
+        assert len([r for r in rows if len(r) == 2]) == 2 and sum(r in weights for r in rows) == 1, rows
