@@ -126,6 +126,7 @@ def _load() -> C.CDLL:
                                                   fp, i64, i64, vp, i64, fp, vp]
     lib.coda_b200_advance_steps.argtypes = [vp, i64, vp]
     lib.coda_b200_selftest_bounded_wait.argtypes = [i32, vp, vp, vp]
+    lib.coda_b200_selftest_int8_wait.argtypes = [i32, vp, vp, vp]
     lib.coda_b200_host_topk_f32.argtypes = [vp, i32, i32, i32, i32, vp]
     lib.coda_b200_host_topk_i64.argtypes = [vp, i32, i32, i32, i32, vp]
     for name in EXPORTS:
@@ -151,7 +152,7 @@ EXPORTS = (
     "coda_b200_attend", "coda_b200_select_candidates", "coda_b200_route_scratch_bytes",
     "coda_b200_route_block", "coda_b200_route_block_phase", "coda_b200_route_static_scratch_bytes", "coda_b200_route_block_noalloc",
     "coda_b200_add_rms_norm", "coda_b200_quantize_rows", "coda_b200_dequantize_rows", "coda_b200_int8_gemm",
-    "coda_b200_advance_steps", "coda_b200_selftest_bounded_wait", "coda_b200_host_topk_f32",
+    "coda_b200_advance_steps", "coda_b200_selftest_bounded_wait", "coda_b200_selftest_int8_wait", "coda_b200_host_topk_f32",
     "coda_b200_host_topk_i64",
 )
 

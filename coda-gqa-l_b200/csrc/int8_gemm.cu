@@ -95,16 +95,16 @@ __device__ __forceinline__ uint32_t ig_try(uint32_t bar, uint32_t parity) {
                : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok;
 }
-__device__ __noinline__ void ig_wait_slow(uint32_t bar, uint32_t parity, int* status, int code, int* abort) {
-  for (int it = 0; it < tma::WAIT_LIMIT; ++it) {
+__device__ __noinline__ void ig_wait_slow(uint32_t bar, uint32_t parity, int* status, int code, int* abort, int limit) {
+  for (int it = 0; it < limit; ++it) {
     if (ig_try(bar, parity)) return;
     if ((it & 15) == 15 && *reinterpret_cast<volatile int*>(abort) != 0) return;
   }
   *reinterpret_cast<volatile int*>(abort) = code;
   if (status) atomicCAS(status, 0, code);
 }
-__device__ __forceinline__ void ig_wait(uint32_t bar, uint32_t parity, int* status, int code, int* abort) {
-  if (!ig_try(bar, parity)) ig_wait_slow(bar, parity, status, code, abort);
+__device__ __forceinline__ void ig_wait(uint32_t bar, uint32_t parity, int* status, int code, int* abort, int limit = tma::WAIT_LIMIT) {
+  if (!ig_try(bar, parity)) ig_wait_slow(bar, parity, status, code, abort, limit);
 }
 // The converged warp waits: one lane polls.
 __device__ __forceinline__ void ig_wait_warp(uint32_t bar, uint32_t parity, int* status, int code, int* abort) {
@@ -485,6 +485,34 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant
   }
 }
 
+// Self-test of these waits, on barriers that nobody arrives at: warp 0 gives up after `poll_limit` polls, warp 1, with the
+// full limit, as soon as it sees the abort word; then every thread passes ig_settle.
+__global__ void ig_selftest_kernel(int poll_limit, int* status, int* report) {
+  __shared__ uint64_t bars[2];
+  __shared__ int s_abort;
+  if (threadIdx.x == 0) {
+    s_abort = 0;
+    tma::mbar_init(&bars[0], 1);
+    tma::mbar_init(&bars[1], 1);
+    tma::fence_barrier_init();
+  }
+  __syncthreads();
+  const int who = threadIdx.x / 32;
+  const long long t0 = clock64();
+  if (who == 0) {
+    if (ig_elect()) ig_wait(smem_u32(&bars[0]), 0, status, 48, &s_abort, poll_limit);
+    __syncwarp();
+  } else ig_wait_warp(smem_u32(&bars[1]), 0, status, 49, &s_abort);
+  const long long dt = clock64() - t0;
+  if (threadIdx.x % 32 == 0) {
+    report[2 * who] = (int)ig_try(smem_u32(&bars[who]), 0);
+    report[2 * who + 1] = dt > 0x7fffffffLL ? 0x7fffffff : (int)dt;
+  }
+  __syncthreads();
+  ig_settle(&s_abort);
+  if (threadIdx.x == 0) report[4] = s_abort;
+}
+
 // ---- launch ----------------------------------------------------------------------------------------------
 struct Int8Plan { bool pair; int nt, split, smem; };   // smem: bytes a CTA of the split kernel may use
 
@@ -618,4 +646,12 @@ extern "C" int coda_b200_int8_gemm(int32_t dtype, int32_t M, int32_t K, int32_t 
   const Int8Operands o{x, x_rs, w, w_rs};
   if (dtype == CODA_F32) return launch_plan<float>(choose_plan(M, K, N), o, p, (cudaStream_t)stream);
   return launch_plan<bf16>(choose_plan(M, K, N), o, p, (cudaStream_t)stream);
+}
+
+extern "C" int coda_b200_selftest_int8_wait(int32_t poll_limit, int32_t* status, int32_t* report, coda_stream_t stream) {
+  CODA_REQUIRE(status && report, CODA_ERR_ARG, "selftest_int8_wait: null pointer");
+  CODA_REQUIRE(poll_limit > 0 && poll_limit <= (1 << 16), CODA_ERR_ARG, "selftest_int8_wait: poll_limit must be in 1..65536");
+  ig_selftest_kernel<<<1, 64, 0, (cudaStream_t)stream>>>(poll_limit, status, report);
+  CODA_CHECK_LAUNCH("selftest_int8_wait");
+  return CODA_OK;
 }

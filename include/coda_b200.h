@@ -480,6 +480,8 @@ int coda_b200_advance_steps(int64_t* step_dev, int64_t n, coda_stream_t stream);
  * report: device int32[5] = {thread 0 saw its barrier complete (0), its cycles, thread 32 saw its barrier complete (0),
  * its cycles, the abort word (77)}.  Returns after the launch like every other entry point. */
 int coda_b200_selftest_bounded_wait(int32_t poll_limit, int32_t* status, int32_t* report, coda_stream_t stream);
+/* The same of the waits of coda_b200_int8_gemm, which are its own (code 48 instead of 77). */
+int coda_b200_selftest_int8_wait(int32_t poll_limit, int32_t* status, int32_t* report, coda_stream_t stream);
 
 /* Host-only helpers (no GPU needed): the selection order used by select_candidates and by
  * the LRU victim ranking, exposed so that CPU tests can compare it with torch.topk. */

@@ -236,3 +236,22 @@ def test_c_entries_refuse_addresses_between_two_elements():
     for scales in ((two, ok), (ok, two)):
         refused(lib.coda_b200_int8_gemm(1, 4, 64, 8, ok, 64, scales[0], ok, 64, scales[1], None, None, 0, ok, 8, 0, None, None))
     refused(lib.coda_b200_int8_gemm(1, 4, 64, 8, ok, 64, ok, ok, 64, ok, None, None, 0, ok, 8, 0, two, None))
+
+
+@pytest.mark.gpu
+def test_a_wait_of_the_product_that_runs_out_reports_and_releases_the_cta():
+    """The bounded wait of the 8-bit product on barriers nobody arrives at: the short one gives up and leaves its code in the
+    status word and the CTA's abort word, the long one of the same CTA leaves on seeing that; the context stays usable."""
+    from coda_gqa_l_b200._lib import check, lib
+    s = torch.cuda.current_stream().cuda_stream
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    report = torch.full((5,), -1, dtype=torch.int32, device="cuda")
+    check(lib.coda_b200_selftest_int8_wait(2048, status.data_ptr(), report.data_ptr(), s), "coda_b200_selftest_int8_wait")
+    torch.cuda.synchronize()
+    r = report.tolist()
+    assert int(status) == 48 and r[0] == 0 and r[2] == 0 and r[4] == 48, r
+    assert r[3] <= 4 * r[1] + 100_000, r                       # (released by the abort word, not by its own limit 2048 times as long)
+    assert float((torch.ones(8, device="cuda") * 2).sum()) == 16.0
+    for limit, st, rep in ((0, status, report), (65537, status, report)):
+        with pytest.raises(RuntimeError):
+            check(lib.coda_b200_selftest_int8_wait(limit, st.data_ptr(), rep.data_ptr(), None), "coda_b200_selftest_int8_wait")
