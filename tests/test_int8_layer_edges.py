@@ -25,9 +25,121 @@ def watch_native(mod):
     return taken
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kw", BF16)
+@pytest.mark.parametrize("bias", [False, True])
+def test_native_step_is_its_projections_called_one_by_one(dtype, kw, bias):
+    """step(x), step(rows in 8 bits) and step_residual(x) of hidden states as a decoding loop has them, each as one native call:
+    the bits of the projections called one by one, the residual added before the result is rounded."""
+    from coda_gqa_l_b200 import _deep_copy_state, quantize_int8
+    mod = layer(kw, dtype)
+    D, B = kw["embed_dim"], 3
+    if bias:
+        mod.o_proj.bias = torch.nn.Parameter(torch.randn(D, device="cuda").to(dtype))
+    ref = piecewise(mod)
+    taken = watch_native(mod)
+    x = hidden(B, 120, D, dtype, 1)
+    torch.manual_seed(2)
+    sa = mod.init_state(batch_size=B, device="cuda", dtype=dtype)
+    sb = _deep_copy_state(sa)
+    for s, m in ((sa, mod), (sb, ref)):
+        m.prefill_chunked(x[:, :40], s, block_size=16)
+    for t in range(40, 120):
+        xt = x[:, t:t + 1].contiguous()
+        if t % 3 == 0:
+            y, want = mod.step_residual(xt, sa), ref._step_fused(ref._cfg(B, dtype, sb), xt, sb, ring(sb), host_update=True, residual=xt)
+        elif t % 3 == 1:
+            y, want = mod.step(xt, sa)[0], ref.step(xt, sb)[0]
+        else:
+            y, want = mod.step(quantize_int8(xt), sa)[0], ref.step(xt, sb)[0]
+        assert torch.equal(y, want), t
+    assert taken[0] == 80
+    for f in FIELDS:
+        assert torch.equal(getattr(sa, f), getattr(sb, f)), f
+    assert (sa.pos, sa.recent_idx, sa.recent_filled) == (sb.pos, sb.recent_idx, sb.recent_filled) and mod.device_status() == 0
+
+
 def ring(st):
     from coda_gqa_l_b200._lib import RingPos
     return RingPos(int(st.pos), int(st.recent_idx), int(st.recent_filled), None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kw", SHAPES)
+@pytest.mark.parametrize("residual", [True, False])
+def test_stack_without_norms_eager_and_captured(dtype, kw, residual):
+    """Prefill, eager, captured and host-fed steps of a stack of 8-bit layers without norms against the layers' projections
+    called one by one.  (An eager float32 step has no native call: its residual is an addition of its own.)"""
+    from coda_gqa_l_b200 import _deep_copy_state
+    st = stack(kw, dtype, 3, True, residual, norms=False)
+    refs = [piecewise(l) for l in st.layers]
+    taken = [watch_native(l) for l in st.layers]
+    native = dtype == torch.bfloat16
+    B, D = 2, kw["embed_dim"]
+    x = hidden(B, 100, D, dtype, 7)
+    torch.manual_seed(3)
+    s1 = st.init_states(batch_size=B, device="cuda", dtype=dtype)
+    s2, s3, s4 = ([_deep_copy_state(s) for s in s1] for _ in range(3))
+
+    def by_hand(h, states, eager):
+        for r, s in zip(refs, states):
+            if eager and not native:
+                h = r.step_residual(h, s) if residual else r.step(h, s)[0]
+            else:
+                h = r.step_graphable(h, s, ring(s), residual=h if residual else None)
+                r.advance_host_scalars(s)
+        return h
+
+    a, c = st.prefill(x[:, :70], s1, block_size=24), st.prefill(x[:, :70], s3, block_size=24)
+    for states in (s2, s4):
+        b = x[:, :70]
+        for r, s in zip(refs, states):
+            b = r.prefill_chunked_residual(b, s, block_size=24) if residual else r.prefill_chunked(b, s, block_size=24)[0]
+        assert torch.equal(a, b) and torch.equal(c, b)
+    for t in range(70, 90):
+        xt = x[:, t:t + 1].contiguous()
+        assert torch.equal(st.step(xt, s1), by_hand(xt, s2, True)), t
+        c = st.step_graph(xt, s3) if t % 2 else st.step_graph_host(xt.cpu(), s3)
+        torch.cuda.synchronize()
+        assert torch.equal(c.cuda(), by_hand(xt, s4, False)), t
+    if native:
+        assert all(n[0] >= 20 for n in taken)
+    for got, want in ((s1, s2), (s3, s4)):
+        for f in FIELDS:
+            assert all(torch.equal(getattr(p, f), getattr(q, f)) for p, q in zip(got, want)), f
+    assert all(l.device_status() == 0 for l in st.layers)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kw", SHAPES)
+def test_stack_hands_its_layers_the_norm_in_64_bits(dtype, kw):
+    """What each layer of a pre-norm stack is given, against the norm of the residual stream in 64 bits (weight and eps its own)."""
+    st = stack(kw, dtype, 3, True)
+    for i, n in enumerate(st.norms):
+        n.eps = 1e-3 * 10 ** i
+    B, D = 2, kw["embed_dim"]
+    x = hidden(B, 12, D, dtype, 7)
+    torch.manual_seed(3)
+    states = st.init_states(batch_size=B, device="cuda", dtype=dtype)
+    seen = []
+
+    def spy(call):
+        def inner(n, s, **k):
+            y, s = call(n, s, **k)
+            seen.append((n, y))
+            return y, s
+        return inner
+
+    for l in st.layers:
+        l.prefill_chunked, l.step = spy(l.prefill_chunked), spy(l.step)
+    for call, xs in ((lambda v: st.prefill(v, states, block_size=4), x[:, :9]), (lambda v: st.step(v, states), x[:, 9:10])):
+        out, h, y = call(xs), xs, None
+        for (q, following), norm in zip(seen, st.norms):
+            s = h.double() if y is None else h.double() + y.double()              # (not yet rounded to the type)
+            check_int8(q, s * torch.rsqrt(s.square().mean(-1, keepdim=True) + norm.eps) * norm.weight.double())
+            h, y = (h if y is None else (h.float() + y.float()).to(dtype)), following
+        assert len(seen) == 3 and torch.equal(out, h + y)
+        seen.clear()
 
 
 def fresh_like(mod, kw, dtype):
