@@ -1187,6 +1187,8 @@ class CoDAGQALandmarkPerf2(nn.Module):
             return y.view(B, L, -1)
         if residual is None:
             return self.o_proj(heads)
+        if type(self.o_proj) is not nn.Linear or self.o_proj.bias is not None:
+            return self.o_proj(heads) + residual
         return torch.addmm(residual.reshape(B * L, -1), heads.reshape(B * L, HD), self.o_proj.weight.t()).view(B, L, -1)
 
     def _step_fused(self, cfg, x, state, rp: RingPos, host_update: bool, routed: bool = False,

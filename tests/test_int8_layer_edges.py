@@ -555,3 +555,31 @@ def test_a_capture_without_copies_quantises_each_weight_once(monkeypatch):
         with torch.cuda.graph(graph):
             call()
         assert len([r for r in rows if len(r) == 2]) == 2 and sum(r in weights for r in rows) == 1, rows
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,kw", SHAPES[:2])
+@pytest.mark.parametrize("int8", [True, False])
+def test_an_output_bias_is_added_beside_a_residual(dtype, kw, int8):
+    """Prefill with the residual taken by the output projection, and the captured step of a stack, with a bias there: what the
+    layer gives plus the residual (a rounding more)."""
+    from coda_gqa_l_b200 import CoDAStack, _deep_copy_state
+    mod = layer(kw, dtype, int8=int8)
+    with torch.no_grad():
+        mod.o_proj.bias = torch.nn.Parameter(torch.linspace(-8, 8, kw["embed_dim"], device="cuda").to(dtype))
+    x = hidden(2, 90, kw["embed_dim"], dtype, 3)
+    torch.manual_seed(2)
+    s1 = mod.init_state(batch_size=2, device="cuda", dtype=dtype)
+    s2 = _deep_copy_state(s1)
+
+    def near(got, y, res):
+        # the plain sum rounds twice and another GEMM may have run: three half steps of either term, fp32 sums of 512 terms
+        u = torch.finfo(dtype).eps / 2
+        bound = (4 * u + 2.0 ** -14) * (y.double().abs() + res.double().abs() + 1)
+        assert bool(((got.double() - y.double() - res.double()).abs() <= bound).all()), float((got.double() - y.double() - res.double()).abs().max())
+
+    near(mod.prefill_chunked_residual(x[:, :80], s1, block_size=16), mod.prefill_chunked(x[:, :80], s2, block_size=16)[0], x[:, :80])
+    st = CoDAStack([mod])
+    for t in range(80, 84):
+        xt = x[:, t:t + 1].contiguous()
+        near(st.step_graph(xt, [s1]), mod.step(xt, s2)[0], xt)
