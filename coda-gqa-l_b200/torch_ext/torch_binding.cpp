@@ -618,7 +618,7 @@ bool is_parameter(PyObject* o) {
   if (PyErr_Occurred()) throw python_error();
   return yes;
 }
-const Tensor& unpack(PyObject* o, const char* what, Role role) {
+Tensor unpack(PyObject* o, const char* what, Role role) {
   TORCH_CHECK_TYPE(THPVariable_Check(o), text("%s: expected a tensor", what));
   const Tensor& t = THPVariable_Unpack(o);
   TORCH_CHECK(!t._fw_grad(/*level=*/0).defined(), text("%s is for inference: it has no derivative (a tensor carries a tangent)", what));
@@ -636,6 +636,11 @@ at::ScalarType unpack_dtype(PyObject* o, const char* what) {
   TORCH_CHECK_TYPE(THPDtype_Check(o), text("%s: unsupported dtype: float32 or bfloat16", what));
   return reinterpret_cast<THPDtype*>(o)->scalar_type;
 }
+// Other threads run while a call works: a launch may wait for room in the stream's queue.
+struct OthersRun {
+  PyThreadState* state = PyEval_SaveThread();
+  ~OthersRun() { PyEval_RestoreThread(state); }
+};
 void arity(Py_ssize_t got, Py_ssize_t want, const char* what) {
   TORCH_CHECK_TYPE(got == want, text("%s: %d arguments expected, got %d", what, int(want), int(got)));
 }
@@ -653,14 +658,17 @@ template <typename... T> PyObject* pack(const T&... t) {
 PyObject* py_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   arity(n, 1, "quantize_int8");
-  auto [q, scale] = quantize_int8(unpack(a[0], "quantize_int8", EITHER));
+  const Tensor x = unpack(a[0], "quantize_int8", EITHER);
+  auto [q, scale] = [&] { const OthersRun run; return quantize_int8(x); }();
   return pack(THPVariable_Wrap(std::move(q)), THPVariable_Wrap(std::move(scale)));
   END_HANDLE_TH_ERRORS
 }
 PyObject* py_dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   arity(n, 3, "dequantize");
-  return THPVariable_Wrap(dequantize_int8(unpack(a[0], "dequantize", ACTIVATION), unpack(a[1], "dequantize", ACTIVATION), unpack_dtype(a[2], "dequantize")));
+  const Tensor values = unpack(a[0], "dequantize", ACTIVATION), scale = unpack(a[1], "dequantize", ACTIVATION);
+  const at::ScalarType dtype = unpack_dtype(a[2], "dequantize");
+  return THPVariable_Wrap([&] { const OthersRun run; return dequantize_int8(values, scale, dtype); }());
   END_HANDLE_TH_ERRORS
 }
 // (x, weight, residual or None, eps, int8) -> (y, sum) or (values, scale, sum); the sum is x itself without a residual
@@ -668,7 +676,7 @@ PyObject* py_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   const char* what = "add_rms_norm";
   arity(n, 5, what);
-  const Tensor& x = unpack(a[0], what, ACTIVATION);
+  const Tensor x = unpack(a[0], what, ACTIVATION), weight = unpack(a[1], what, WEIGHT);
   const OptTensor residual = unpack_opt(a[2], "add_rms_norm: residual", ACTIVATION);
   const double eps = PyFloat_AsDouble(a[3]);
   if (PyErr_Occurred()) throw python_error();
@@ -676,7 +684,10 @@ PyObject* py_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int int8 = PyObject_IsTrue(a[4]);
   if (int8 < 0) throw python_error();
   Tensor y, q, scale, sum;
-  norm(x, unpack(a[1], what, WEIGHT), residual, eps, int8 ? nullptr : &y, int8 ? &q : nullptr, int8 ? &scale : nullptr, &sum);
+  {
+    const OthersRun run;
+    norm(x, weight, residual, eps, int8 ? nullptr : &y, int8 ? &q : nullptr, int8 ? &scale : nullptr, &sum);
+  }
   PyObject* total = residual.has_value() ? THPVariable_Wrap(std::move(sum)) : Py_NewRef(a[0]);
   return int8 ? pack(THPVariable_Wrap(std::move(q)), THPVariable_Wrap(std::move(scale)), total) : pack(THPVariable_Wrap(std::move(y)), total);
   END_HANDLE_TH_ERRORS
@@ -687,9 +698,12 @@ PyObject* py_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   arity(n, 9, what);
   const int ready = PyObject_IsTrue(a[8]);
   if (ready < 0) throw python_error();
-  return THPVariable_Wrap(int8_linear(unpack(a[0], what, ACTIVATION), unpack(a[1], what, ACTIVATION), unpack(a[2], what, WEIGHT), unpack(a[3], what, WEIGHT),
-                                      unpack_opt(a[4], what, WEIGHT), unpack_opt(a[5], "int8_linear: residual", ACTIVATION), unpack_dtype(a[6], what),
-                                      unpack_opt(a[7], what, WEIGHT), ready != 0));
+  const Tensor x = unpack(a[0], what, ACTIVATION), x_scale = unpack(a[1], what, ACTIVATION);
+  const Tensor w = unpack(a[2], what, WEIGHT), w_scale = unpack(a[3], what, WEIGHT);
+  const OptTensor bias = unpack_opt(a[4], what, WEIGHT), residual = unpack_opt(a[5], "int8_linear: residual", ACTIVATION);
+  const at::ScalarType dtype = unpack_dtype(a[6], what);
+  const OptTensor status = unpack_opt(a[7], what, WEIGHT);
+  return THPVariable_Wrap([&] { const OthersRun run; return int8_linear(x, x_scale, w, w_scale, bias, residual, dtype, status, ready != 0); }());
   END_HANDLE_TH_ERRORS
 }
 

@@ -255,3 +255,41 @@ def test_a_wait_of_the_product_that_runs_out_reports_and_releases_the_cta():
     for limit, st, rep in ((0, status, report), (65537, status, report)):
         with pytest.raises(RuntimeError):
             check(lib.coda_b200_selftest_int8_wait(limit, st.data_ptr(), rep.data_ptr(), None), "coda_b200_selftest_int8_wait")
+
+
+@pytest.mark.gpu
+def test_a_call_that_waits_for_room_in_the_queue_lets_other_threads_run():
+    """More launches than the queue of a busy stream holds: while they wait, other Python threads go on (one may hold what the
+    stream is waiting for)."""
+    import threading
+    import time
+
+    from coda_gqa_l_b200 import add_rms_norm, int8_linear, quantize_int8
+    x, w = torch.randn(4, 64, device="cuda"), torch.ones(64, device="cuda")
+    p = quantize_int8(torch.randn(8, 64, device="cuda"))
+    gap, stop = [0.0], threading.Event()
+
+    def tick():
+        last = time.perf_counter()
+        while not stop.is_set():
+            time.sleep(0.001)
+            now = time.perf_counter()
+            gap[0], last = max(gap[0], now - last), now
+
+    q = quantize_int8(x)
+    int8_linear(q, p), q.dequantize(), add_rms_norm(x, w)
+    for call in (lambda: quantize_int8(x), lambda: q.dequantize(), lambda: add_rms_norm(x, w), lambda: int8_linear(q, p)):
+        torch.cuda.synchronize()
+        gap[0] = 0.0
+        stop.clear()
+        thread = threading.Thread(target=tick)
+        thread.start()
+        torch.cuda._sleep(1_200_000_000)                        # some 0.6 s
+        t0 = time.perf_counter()
+        for _ in range(3000):
+            call()
+        waited = time.perf_counter() - t0
+        stop.set()
+        thread.join()
+        assert waited > 0.3 and gap[0] < 0.2, (waited, gap[0])
+    torch.cuda.synchronize()
