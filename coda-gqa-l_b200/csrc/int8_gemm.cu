@@ -124,7 +124,7 @@ __device__ __forceinline__ void ig_settle(const int* abortw) {
 // With few tokens the product is one pass over the weights, bound by HBM: what counts is that every SM loads its share.
 // A tile is 128 channels by NT tokens, and the S CTAs of a cluster take equal runs of its K.  The partial sums are integers:
 // any order gives the same bits.  They meet through distributed shared memory, each CTA finishing `per` of the tokens.
-// Back to back on cold weights: 32 x 4096 -> 6177 8.5 us, 1 x 512 -> 777 2.5 us; what grows with the size does so at the HBM's
+// Back to back on cold weights: 32 x 4096 -> 6177 9.1 us, 1 x 512 -> 777 2.5 us; what grows with the size does so at the HBM's
 // rate (8192 x 8192 weights 13.2 us, 4096 x 4096 6.1: 50 MB in 7.1 us), some 3.5 us do not.
 // Warp 0 = TMA producer, warp 1 = MMA issuer and TMEM owner, warps 2-5 = epilogue; residual and scales of the epilogue are
 // in shared memory before the last MMA is done.
@@ -305,8 +305,8 @@ int8_split_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constan
 // ---- many tokens: pairs of SMs ------------------------------------------------------------------------
 // A pair of CTAs works on 256 channels x NT tokens with one MMA (cta_group::2, M = 256): each holds its 128 channels and
 // half of the tokens, so a stage costs 128 + NT / 2 rows of loads for 128 x NT products a byte of K -- two thirds of what
-// one CTA alone would load for its 128 x NT, which is what the L2 cannot feed (it gives some 13 TB/s).  8192 x 8192 -> 8192 323
-// us = 3.4 POP/s, 340 with a residual; 16384 x 4096 -> 6177 275 us; the tensor pipe is 87 % active.  The pairs walk over the tiles
+// one CTA alone would load for its 128 x NT, which is what the L2 cannot feed (it gives some 13 TB/s).  8192 x 8192 -> 8192
+// with a residual 330 - 365 us (3.3 - 3.0 POP/s, as the power cap lets it); 16384 x 4096 -> 6177 276 us; the tensor pipe is 87 % active.  The pairs walk over the tiles
 // (persistent); the accumulator is double-buffered in TMEM, so a tile's epilogue runs under the next tile's MMAs.
 // Warp 0 = TMA producer (its copies complete on the pair's first CTA's barrier), warp 1 = MMA issuer (first CTA only) and
 // TMEM owner, warps 2-9 = epilogue, two warps per 32 channels with half of the tokens each.
@@ -592,19 +592,19 @@ int launch_plan(const Int8Plan& q, const Int8Operands& o, Int8GemmParams p, cuda
 
 // The plan that is estimated to be the quickest.  Microseconds beyond what every plan costs, fitted to every plan's time at
 // 1008 sizes (M 1 .. 4096, K 128 .. 8192, N 200 .. 20000, bf16, back to back with cold weights): a k-block costs a CTA or pair
-// so much, waves of tiles follow one another, and HBM time adds to that as the other leg of a right angle.  What it chooses
-// there is 0.2 % slower than the best plan in the geometric mean, 11 % at worst.
+// so much, waves of tiles follow one another, and the bytes that go in and out, at a rate that was fitted with the rest (twice
+// what HBM gives: loads and products overlap), add to that as the other leg of a right angle.
 Int8Plan choose_plan(long long M, long long K, long long N) {
   auto up = [](long long a, long long b) { return (a + b - 1) / b; };
   const long long nkb = up(K, IG_BK);
-  const double hbm = (double)(N * K + M * K + 2 * M * N) / 13.3e6;
+  const double bytes = (double)(N * K + M * K + 2 * M * N) / 13.3e6;
   Int8Plan best = {};
   double least = 1e30;
   for (int i = 0; i < 3; ++i) {                            // pairs of SMs, 74 of them
     static const double block[3] = {0.163, 0.185, 0.279}, tail[3] = {1.06, 1.23, 1.45};
     const int nt = 64 << i;
     const double run = (double)up(up(N, 2 * IG_BN) * up(M, nt), 74) * fmax((double)up(nkb, ip_kps(nt)) * ip_kps(nt) * block[i], tail[i]);
-    const double t = sqrt(run * run + hbm * hbm) + tail[i];
+    const double t = sqrt(run * run + bytes * bytes) + tail[i];
     if (t < least) { least = t; best = Int8Plan{true, nt, 1, 0}; }
   }
   if (M > 512) return best;
@@ -617,7 +617,7 @@ Int8Plan choose_plan(long long M, long long K, long long N) {
     if (split == 8 && half) break;
     const double waves = (double)up(ctas, resident[at] * (half ? 2 : 1));
     const double run = waves * (double)(up(up(nkb, IS_KPS), split) * IS_KPS) * block[i] * (half && ctas > 148 ? 3.1 : 1.0);
-    const double t = sqrt(run * run + hbm * hbm) + 1.47 * (waves - 1) + (split == 1 ? tail1[i] : tail[i]);
+    const double t = sqrt(run * run + bytes * bytes) + 1.47 * (waves - 1) + (split == 1 ? tail1[i] : tail[i]);
     if (t < least) { least = t; best = Int8Plan{false, nt, split, half ? IS_SMEM_HALF : IS_SMEM_WHOLE}; }
   }
   return best;

@@ -9,9 +9,9 @@
 // becomes zeros with scale NaN, so that whatever is computed from it is NaN.
 // Bound: HBM (x, residual, s, one byte of q an element), and for the rows of a decode step the latency of one load,
 // two reductions and one store.  So a row stays in the registers of the threads that loaded it: one pass over memory.
-// 16384 x 4096 bf16: norm with residual to 8 bits 71 us = 6.6 TB/s (1.01 of the measured copy), rows to 8 bits 33 us = 6.2, back
-// 34 us = 5.8; 32 x 4096 about 2 us each.  Rows that are no whole vectors: 58 us for the norm of 8192 x 4094 bf16 (36 where
-// they are), 76 us for 8192 x 4095 (120 before odd rows were read by aligned words).
+// 16384 x 4096 bf16: norm with residual to 8 bits 69 us = 6.8 TB/s (1.04 of the measured copy), rows to 8 bits 33 us = 6.1, back
+// 34 us = 5.8; 32 x 4096 under 2 us each.  Rows that are no whole vectors: 57 us for the norm of 8192 x 4094 bf16 (36 where
+// they are), 72 us for 8192 x 4095 (120 before odd rows were read by aligned words).
 #include "coda_common.cuh"
 #include <type_traits>
 
