@@ -306,7 +306,7 @@ int8_split_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constan
 // A pair of CTAs works on 256 channels x NT tokens with one MMA (cta_group::2, M = 256): each holds its 128 channels and
 // half of the tokens, so a stage costs 128 + NT / 2 rows of loads for 128 x NT products a byte of K -- two thirds of what
 // one CTA alone would load for its 128 x NT, which is what the L2 cannot feed (it gives some 13 TB/s).  8192 x 8192 -> 8192
-// with a residual 330 - 365 us (3.3 - 3.0 POP/s, as the power cap lets it); 16384 x 4096 -> 6177 276 us; the tensor pipe is 87 % active.  The pairs walk over the tiles
+// with a residual 330 - 365 us (3.3 - 3.0 POP/s, as the power cap lets it); 16384 x 4096 -> 6177 276 us; the tensor pipe is 84 to 87 % active.  The pairs walk over the tiles
 // (persistent); the accumulator is double-buffered in TMEM, so a tile's epilogue runs under the next tile's MMAs.
 // Warp 0 = TMA producer (its copies complete on the pair's first CTA's barrier), warp 1 = MMA issuer (first CTA only) and
 // TMEM owner, warps 2-9 = epilogue, two warps per 32 channels with half of the tokens each.
