@@ -251,6 +251,16 @@ class CoDAGQALandmarkPerf2(nn.Module):
         self.use_torch_ops = False
         self._status = None
 
+    def __getstate__(self):
+        """For copies and ``torch.save``: the layer without what it derives from its parameters and keeps for its calls
+        (addresses, copies, scratch), which a copy makes for itself."""
+        d = self.__dict__.copy()
+        d.update(_cfg_cache={}, _const_cache={}, _scratch={}, _recorded={}, _gemm_ok={}, _fused=None, _fused_ptrs=[], _wt=None,
+                 _qrec=None, _status=None, _int8=None, _int8_rows=None)
+        for name in ("_bundle", "_bundle8"):
+            d.pop(name, None)
+        return d
+
     # ------------------------------------------------------------------ state
     def init_state(self, *, batch_size: int, device, dtype: torch.dtype,
                    mem_init: Optional[str] = None) -> CoDAGQALandmarkStatePerf2:

@@ -68,6 +68,10 @@ class CoDAStack(nn.Module):
         # launches chained by programmatic dependent launch measure faster (1.21 against 1.32 ms per C4 step).
         self.chain_projections = False
 
+    def __getstate__(self):
+        """For copies and ``torch.save``: without the captured step, which belongs to these layers and their states."""
+        return self.__dict__ | {"_graph": None, "_watch": None}
+
     def init_states(self, *, batch_size: int, device, dtype) -> List[CoDAGQALandmarkStatePerf2]:
         return [l.init_state(batch_size=batch_size, device=device, dtype=dtype) for l in self.layers]
 

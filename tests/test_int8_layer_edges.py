@@ -583,3 +583,53 @@ def test_an_output_bias_is_added_beside_a_residual(dtype, kw, int8):
     for t in range(80, 84):
         xt = x[:, t:t + 1].contiguous()
         near(st.step_graph(xt, [s1]), mod.step(xt, s2)[0], xt)
+
+
+@pytest.mark.parametrize("int8", [True, False])
+def test_a_used_layer_can_be_copied_and_saved(int8, monkeypatch):
+    """After the eager step's addresses were gathered: a deep copy and a saved and loaded layer have the parameters and
+    switches, and make their own copies of the weights."""
+    import copy
+    import io
+    mod = on_cpu(monkeypatch)
+    mod.use_int8_projections = int8
+    gather = lambda m: (m._int8_bundle if int8 else m._decode_bundle)(torch.device("cpu"), torch.float32)  # noqa: E731
+    with torch.no_grad():
+        mine = gather(mod)
+        buf = io.BytesIO()
+        torch.save(mod, buf)
+        buf.seek(0)
+        for other in (copy.deepcopy(mod), torch.load(buf, weights_only=False)):
+            assert other.use_int8_projections == int8
+            for (n, p), (m, q) in zip(mod.named_parameters(), other.named_parameters()):
+                assert n == m and torch.equal(p, q) and p.data_ptr() != q.data_ptr()
+            theirs = gather(other)
+            assert theirs["layer"].bias != mine["layer"].bias
+            other.o_proj.weight.mul_(2.0)
+            assert gather(other) is not theirs and gather(mod) is mine
+
+
+@pytest.mark.gpu
+def test_a_used_stack_can_be_copied():
+    """A stack whose step has been captured: the copy captures its own and gives the same results."""
+    import copy
+
+    from coda_gqa_l_b200 import _deep_copy_state
+    dtype, kw = SHAPES[1]
+    st = stack(kw, dtype, 2, True)
+    x = hidden(2, 6, kw["embed_dim"], dtype, 3)
+    torch.manual_seed(2)
+    s1 = st.init_states(batch_size=2, device="cuda", dtype=dtype)
+    st.step_graph(x[:, :1], s1)
+    st.step(x[:, 1:2], s1)
+    other = copy.deepcopy(st)
+    s2 = [_deep_copy_state(s) for s in s1]
+    for t in range(2, 6):
+        a, b = st.step_graph(x[:, t:t + 1], s1), other.step_graph(x[:, t:t + 1], s2)
+        torch.cuda.synchronize()
+        assert torch.equal(a, b)
+    with torch.no_grad():
+        other.layers[0].o_proj.weight.mul_(-1.0)
+    a, b = st.step_graph(x[:, :1], s1), other.step_graph(x[:, :1], s2)
+    torch.cuda.synchronize()
+    assert not torch.equal(a, b)
