@@ -56,6 +56,8 @@ def _stream(device: Optional[torch.device] = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
+
 _SIDE_STREAMS: dict = {}
 
 
@@ -207,7 +209,7 @@ class CoDAGQALandmarkPerf2(nn.Module):
         self._fused = None
         self._fused_ptrs = []
         self._wt = None
-        self._recorded: Dict[int, torch.Tensor] = {}
+        self._recorded: Dict[tuple, object] = {}       # what graphs captured around the layer read
         # When set to a list, every attention launch appends (Lq, start_event, end_event) to it.
         self.kernel_timers = None
         self._qrec = None
@@ -491,6 +493,8 @@ class CoDAGQALandmarkPerf2(nn.Module):
                self.summary_eta_logit._version, self.rope.inv_freq.data_ptr(), _p(nw), 0 if nw is None else nw._version)
         hit = self._const_cache.get("k")
         if hit is not None and hit[0] == key:
+            if _recording(self.theta):
+                self._pin()
             return hit[1]
         th = self.theta.detach()
         vals = (self.rope.inv_freq.detach().to(device=device, dtype=torch.float32).contiguous(),
@@ -502,6 +506,13 @@ class CoDAGQALandmarkPerf2(nn.Module):
             _settle(th)
             self._const_cache["k"] = (key, vals)
         return vals
+
+    def _pin(self) -> None:
+        """The graph that is being captured holds addresses of the derived copies as they are: they stay as long as the layer,
+        or as whoever keeps them with the graph."""
+        for copies in (self._fused, self._wt, self._int8, self._const_cache.get("k")):
+            if copies is not None:
+                self._recorded["copies", id(copies)] = copies
 
     def _fused_weight(self):
         """One [q | k | v | lambda | gate | pad] weight so that the five input projections are a single GEMM.
@@ -537,7 +548,7 @@ class CoDAGQALandmarkPerf2(nn.Module):
                     to = to[off:off + l.out_features]
                     to.copy_(p.data)
                     if recording:
-                        self._recorded[p.data_ptr()] = p.data
+                        self._recorded["parameter", p.data_ptr()] = p.data
                     else:
                         p.data = to
             off += l.out_features
@@ -1139,13 +1150,13 @@ class CoDAGQALandmarkPerf2(nn.Module):
         """``n`` bytes or more for what a call writes and reads again: calls on one stream follow one another, so they share
         it; calls on two streams, or replays of two graphs, may run side by side."""
         key = (what, device.index, stream)
+        if _capturing():
+            self._pin()                        # (an eager step's addresses were gathered before: nothing else looks)
+            return torch.empty(n, dtype=torch.uint8, device=device)
         kept = self._scratch.get(key)
-        if kept is not None and kept[0] >= n:
-            return kept[1]
-        buf = torch.empty(n, dtype=torch.uint8, device=device)
-        if not _recording(buf):
-            self._scratch[key] = (n, buf)
-        return buf
+        if kept is None or kept[0] < n:
+            kept = self._scratch[key] = (n, torch.empty(n, dtype=torch.uint8, device=device))
+        return kept[1]
 
     def _fused_write_ok(self, cfg, q: Optional[torch.Tensor] = None) -> bool:
         ok = getattr(cfg, "_fused_write", None)

@@ -193,6 +193,7 @@ class CoDAStack(nn.Module):
                   "coda_b200_advance_steps")
             return h
 
+        recorded = [dict(l._recorded) for l in self.layers]
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             out_static = body(x_static)
@@ -220,6 +221,8 @@ class CoDAStack(nn.Module):
                            states=list(states), key=self._graph_key(states, x_static.dtype),
                            expect=[(st.pos, st.recent_idx, st.recent_filled) for st in states],
                            keep=[(l._fused, l._wt, l._int8, l._const_cache.get("k"), l._qrec, l._status) for l in self.layers])
+        for l, before in zip(self.layers, recorded):
+            l._recorded = before                     # (kept with the graphs: another capture lets them go)
 
     def _graph_key(self, states, dtype):
         """What a captured step depends on besides the ring scalars, cheap enough to evaluate before every replay:

@@ -633,3 +633,56 @@ def test_a_used_stack_can_be_copied():
     a, b = st.step_graph(x[:, :1], s1), other.step_graph(x[:, :1], s2)
     torch.cuda.synchronize()
     assert not torch.equal(a, b)
+
+
+def test_copies_that_a_capture_used_stay(monkeypatch):
+    """Derived copies made before a capture are what the graph reads: another set made later does not free them."""
+    import weakref
+
+    from coda_gqa_l_b200 import attention
+    mod = on_cpu(monkeypatch)
+    mod.use_int8_projections = True
+    cpu = torch.device("cpu")
+
+    def made():
+        mod._int8_weights()
+        t = [mod._fused_weight()[0], mod._skinny_weights()[1], mod._skinny_weights()[2], mod._consts(cpu, torch.float32)[1]]
+        return [weakref.ref(x) for x in t], [x.clone() for x in t]
+
+    def change():
+        with torch.no_grad():
+            set_key(mod)
+            mod.o_proj.weight.mul_(0.5)
+            mod.theta.add_(0.1)
+        return made()
+
+    with torch.no_grad():
+        seen, values = made()
+        monkeypatch.setattr(attention, "_recording", lambda t: True)
+        made()                                             # what a captured call looks up
+        monkeypatch.setattr(attention, "_recording", lambda t: False)
+        later, _ = change()
+        assert all(r() is not None and torch.equal(r(), v) for r, v in zip(seen, values))
+        change()
+        assert all(r() is not None and torch.equal(r(), v) for r, v in zip(seen, values))
+        assert all(r() is None for r in later[1:])         # (made and used outside: not kept)
+
+
+@pytest.mark.gpu
+def test_a_recaptured_stack_keeps_one_set_of_copies():
+    """Changed weights make a stack capture again; what the graph before read goes with it."""
+    dtype, kw = SHAPES[1]
+    st = stack(kw, dtype, 2, True)
+    x = hidden(2, 1, kw["embed_dim"], dtype, 3)
+    torch.manual_seed(2)
+    s = st.init_states(batch_size=2, device="cuda", dtype=dtype)
+    sizes = []
+    for i in range(6):
+        with torch.no_grad():
+            for l in st.layers:
+                set_key(l)
+        st.step_graph(x, s)
+        torch.cuda.synchronize()
+        sizes.append(torch.cuda.memory_allocated())
+        assert all(not l._recorded for l in st.layers)
+    assert max(sizes[2:]) - min(sizes[2:]) < 2 ** 20, sizes
