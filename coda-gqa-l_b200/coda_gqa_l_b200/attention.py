@@ -602,6 +602,8 @@ class CoDAGQALandmarkPerf2(nn.Module):
         do not see, e.g. through ``.data``)."""
         self._wt = None
         self._int8 = None
+        for name in ("_bundle", "_bundle8"):
+            self.__dict__.pop(name, None)
 
     def _int8_weights(self, f=None):
         """(sources, fused input weight and output weight in 8 bits, fused bias): quantised on first use and again when a

@@ -686,3 +686,22 @@ def test_a_recaptured_stack_keeps_one_set_of_copies():
         sizes.append(torch.cuda.memory_allocated())
         assert all(not l._recorded for l in st.layers)
     assert max(sizes[2:]) - min(sizes[2:]) < 2 ** 20, sizes
+
+
+@pytest.mark.parametrize("int8", [True, False])
+def test_refreshed_weights_are_gathered_again(int8, monkeypatch):
+    """Writes past the version counters, announced by refresh_weights: the eager step's copies are those of the new values."""
+    mod = on_cpu(monkeypatch)
+    mod.use_int8_projections = int8
+    gather = lambda: (mod._int8_bundle if int8 else mod._decode_bundle)(torch.device("cpu"), torch.float32)  # noqa: E731
+    with torch.no_grad():
+        last = gather()
+        for p in (mod.q_proj.weight, mod.o_proj.weight):
+            p.data.mul_(-2.0)
+        mod.refresh_weights()
+        now = gather()
+        assert now is not last
+        if int8:
+            assert torch.equal(now["w"][2].scale, mod.o_proj.weight.abs().amax(1) / 127)
+        else:
+            assert torch.equal(now["w_out_t"], mod.o_proj.weight.t()) and torch.equal(now["w_in_t"], mod._fused_weight()[0].t())
