@@ -77,7 +77,7 @@ __device__ __forceinline__ Q8 row_scale(uint32_t amax) {
 }
 // q = rint(127 y / a), ties to even.  To round, 1.5 * 2^23 is added: its last bit is worth 1, and the low byte of the sum's
 // bits is q.  y * inv is within 127 * 2^-24 of the quotient, so its nearest integer is right unless it lies that close to a
-// half.  A row's largest value being even, half of it is such a tie: without more, 1 of some 6000 values of random bf16 rows
+// half.  Half of a row's largest value is such a tie, 63.5: without more, 1 of some 6000 values of random bf16 rows
 // came out a step off (and 1 of 20000 by a division by the scale: two roundings miss ties too).  How far that is looked at:
 // Q8_SHORT  bf16 rows as they are: a quotient of two 8-bit values is a half or 2 / (512 * 255) away from one at the least (254 y -
 //           256 a is even; further above one half), so y * inv is rounded to multiples of 2^-15 first: that restores the
