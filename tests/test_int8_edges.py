@@ -50,6 +50,22 @@ def test_values_on_a_tie_and_near_one(dim, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_every_quotient_of_two_8_bit_mantissas(dtype):
+    """A row for each mantissa of its largest value, with every mantissa at every exponent that can still round to one or more
+    below it and some under that, both signs: all there is among bfloat16 rows, up to powers of two."""
+    from coda_gqa_l_b200 import quantize_int8
+    m = torch.arange(128, 256, device="cuda").double()
+    below = (m[:, None] * 2.0 ** -torch.arange(0, 14, device="cuda").double()).reshape(-1)
+    y = torch.cat([below, -below])[None, :].expand(128, -1)
+    y = torch.where(y.abs() <= m[:, None], y, torch.zeros_like(y))
+    for scale in (1.0, 2.0 ** -92, 2.0 ** 116):
+        x = (torch.cat([m[:, None], y], dim=1) * scale).to(dtype)
+        assert torch.equal(x.double(), torch.cat([m[:, None], y], dim=1) * scale)
+        assert assert_nearest(x, quantize_int8(x)) >= 2 * 128
+
+
+@pytest.mark.gpu
 def test_single_rows_of_odd_length_are_used_in_place():
     """One row has no distance to another: rows of this package's own making are neither copied nor moved, a product allocates
     its result and nothing else, as it does for two rows."""
