@@ -56,7 +56,7 @@ def test_every_quotient_of_two_8_bit_mantissas(dtype):
     below it and some under that, both signs: all there is among bfloat16 rows, up to powers of two."""
     from coda_gqa_l_b200 import quantize_int8
     m = torch.arange(128, 256, device="cuda").double()
-    below = (m[:, None] * 2.0 ** -torch.arange(0, 14, device="cuda").double()).reshape(-1)
+    below = (m[:, None] * torch.tensor([2.0 ** -i for i in range(14)], device="cuda", dtype=torch.float64)).reshape(-1)
     y = torch.cat([below, -below])[None, :].expand(128, -1)
     y = torch.where(y.abs() <= m[:, None], y, torch.zeros_like(y))
     for scale in (1.0, 2.0 ** -92, 2.0 ** 116):
